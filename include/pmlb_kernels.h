@@ -49,7 +49,9 @@ typedef enum {
   PMLB_F16 = 13,
   PMLB_F32 = 14,
   PMLB_F64 = 15,
-  PMLB_BF16 = 16
+  PMLB_BF16 = 16,
+  PMLB_F8E4M3 = 17, /* 4 exponent and 3 fraction bits, largest value 448, no infinities; operands of block products only */
+  PMLB_F8E5M2 = 18  /* 5 exponent and 2 fraction bits, largest finite value 57344 */
 } pmlb_dtype;
 
 /* Aggregations and combinations of a Tile contraction; values equal plaidml_agg_op /
@@ -459,6 +461,155 @@ pmlb_status pmlb_special_dispatch(const pmlb_special_desc* desc, pmlb_plan** pla
  * may be null, and then only the other is computed. */
 pmlb_status pmlb_special_invoke(pmlb_plan* plan, void* stream, const void* in0, const void* in1, const void* in2,
                                 void* out0, void* out1);
+
+/* ---------------------------------------------------------------- products of 8-bit floats, scaled by blocks
+ * (no counterpart in the reference)
+ *
+ *   C[i, j] = sum_b  a_scale[i, b] * b_scale[j', b] * sum_{k in block b} A[i, k] * B[j, k]
+ *
+ * A [m][k] and B [n][k] hold 8-bit floats (E4M3 or E5M2, each its own), both with k contiguous; block b is the terms
+ * [128 b, 128 b + 128), the last one shorter where 128 does not divide k.  A has a scale for each row and block, B for
+ * each 128 rows and block (b_scale_rows = 128, j' = j / 128: weights) or for each row and block (b_scale_rows = 1, j' = j:
+ * the second operand of a weight gradient).  The 128 products of a block are added on the tensor cores, the blocks, times
+ * their scales, in f32 in the order of b; one rounding to out_dtype (F32, BF16 or F16).  The K range of products of few
+ * rows is shared by up to eight CTAs, which adds 2..8 runs of blocks in a fixed order: results are the same on every call.
+ *
+ * groups = 0: one product.  groups = 1..1024 with `offsets`, int32[groups + 1] in device memory, ascending from 0:
+ *   PMLB_GROUP_ROWS   rows [offsets[g], offsets[g + 1]) of A and C belong to B[g] (stride_b elements apart, scales
+ *                     b_scale_group apart): the experts' products.  m is the number of rows that A and C have; rows from
+ *                     offsets[groups] on are neither computed nor written.
+ *   PMLB_GROUP_TERMS  C[g] (stride_c elements apart) is the product over the terms [offsets[g], offsets[g + 1]) alone:
+ *                     the experts' weight gradients, both operands transposed by PMLB_QUANT_COLUMNS.  Offsets are
+ *                     multiples of 128 (see `align` of pmlb_route_desc); a group without terms gives zeros.
+ * Offsets outside [0, m] (of terms: [0, k]) are taken as the nearest edge; a group that would end before it begins is empty
+ * and, of rows, the next one begins where the last one ended.
+ * lda, ldb and stride_b are multiples of 16 and the operands start on 16 bytes. */
+#define PMLB_GROUP_ROWS 0
+#define PMLB_GROUP_TERMS 1
+
+typedef struct {
+  int32_t a_dtype, b_dtype;          /* PMLB_F8E4M3 or PMLB_F8E5M2 */
+  int32_t out_dtype;                 /* PMLB_F32, PMLB_BF16 or PMLB_F16 */
+  int32_t m, n, k;
+  int32_t groups, group_dim;         /* 0, or the number of groups and PMLB_GROUP_* */
+  int64_t lda, ldb, ldc;             /* elements between rows */
+  int64_t stride_b, stride_c;        /* elements between the groups' B (ROWS) or C (TERMS) */
+  int32_t b_scale_rows;              /* 128 or 1 */
+  int32_t reserved0;
+  int64_t a_scale_row, a_scale_block;/* elements from one row's scale to the next row's / to the next block's */
+  int64_t b_scale_row, b_scale_block, b_scale_group; /* row: of 128 rows of B, or of one */
+} pmlb_block_gemm_desc;
+
+pmlb_status pmlb_block_gemm_dispatch(const pmlb_block_gemm_desc* desc, pmlb_plan** plan);
+/* `offsets` is NULL for groups = 0. */
+pmlb_status pmlb_block_gemm_invoke(pmlb_plan* plan, void* stream, const void* a, const float* a_scale, const void* b,
+                                   const float* b_scale, const int32_t* offsets, void* c);
+
+/* ---------------------------------------------------------------- quantisation by blocks
+ * (no counterpart in the reference)
+ *
+ *   scale = max(amax, 2^-100) / largest      q = to_8_bits(x * (1 / scale))      amax: largest |x| of the block
+ *
+ * with `largest` 448 (E4M3) or 57344 (E5M2), every operation in f32 rounded to nearest, and to_8_bits rounding to nearest
+ * even and saturating.  q * scale stands for x.  A NaN stays NaN and does not count in amax; a block that holds an
+ * infinity has an infinite scale, and stands for NaN.  x: F32, BF16 or F16, [batch][rows][cols].
+ *   PMLB_QUANT_ROWS      blocks of 128 along a row                  q [rows][cols]   scale[row, block of columns]
+ *   PMLB_QUANT_COLUMNS   blocks of 128 down a column, transposed    q [cols][rows]   scale[column, block of rows]
+ *   PMLB_QUANT_TILES     blocks of 128 x 128                        q [rows][cols]   scale[block of rows, block of columns]
+ *   PMLB_QUANT_TILES_TRANSPOSED   the same, transposed              q [cols][rows]   scale[block of columns, block of rows]
+ * scale_row / scale_block are the elements between scales along q's rows (of 128 rows for the tile forms) and along its
+ * blocks of 128 columns.  source_rows > 0 (ROWS, batch 1): row i is row rows[i] / source_div of an x of source_rows rows,
+ * or zeros where rows[i] < 0 or beyond them: `rows` is the `source` of a routing, source_div its top_k. */
+#define PMLB_QUANT_ROWS 0
+#define PMLB_QUANT_COLUMNS 1
+#define PMLB_QUANT_TILES 2
+#define PMLB_QUANT_TILES_TRANSPOSED 3
+
+typedef struct {
+  int32_t in_dtype, out_dtype;
+  int32_t form;                      /* PMLB_QUANT_* */
+  int32_t rows, cols, batch;
+  int64_t ldx, ldq;                  /* elements between rows of x and of q */
+  int64_t stride_x, stride_q;        /* elements between batch entries */
+  int64_t scale_row, scale_block, stride_scale;
+  int32_t source_rows, source_div;
+} pmlb_quant_desc;
+
+pmlb_status pmlb_quant_dispatch(const pmlb_quant_desc* desc, pmlb_plan** plan);
+/* `rows` (int32, device memory) is NULL for source_rows = 0. */
+pmlb_status pmlb_quant_invoke(pmlb_plan* plan, void* stream, const void* x, const int32_t* rows, void* q, float* scale);
+
+/* ---------------------------------------------------------------- routing of tokens to experts
+ * (no counterpart in the reference)
+ *
+ * For each of `tokens` rows z of `experts` logits (F32, BF16 or F16):
+ *   s = softmax(z) or sigmoid(z);   r = s + bias, or, without a bias and with one group, r = z
+ *   experts are `groups` runs of equal length; a group's value is the sum of its two largest r (of its only one); the
+ *   top_groups groups of the largest values stay
+ *   ids = the top_k experts of the largest r in them, in descending order, ties to the lowest index (of the group, too)
+ *   weights[j] = scale * s[ids[j]], with `renormalise` divided by the sum over the token's choices
+ * What is chosen is what these definitions give in 64-bit arithmetic: choices that 32 bits leave open are made again in 64.
+ * NaN counts as minus infinity, a sigmoid below e^-709 as zero; a token whose chosen scores are all zero has
+ * zero weights.  The bias (f32, may be NULL)
+ * takes part in the choice alone.
+ *
+ * The experts' order of the (token, choice) pairs, pair t * top_k + j going to expert ids[t, j] (`rows` > 0, else
+ * the three are not computed and may be NULL):
+ *   offsets  int32[experts + 1]      expert e's segment of rows; its length is a multiple of `align` (1..1024)
+ *   source   int32[rows]             the pair of each row in ascending order within a segment, -1 on the rows that fill
+ *                                    a segment up and on those behind the last one
+ *   position int32[tokens][top_k]    the row of each pair
+ * rows is at least tokens * top_k + min(experts, tokens * top_k) * (align - 1), rounded down to a multiple of align.
+ * experts <= 1024, top_k <= 32, groups <= 32, at most 2^24 pairs.
+ *
+ * pmlb_route_order does the last part for ids that come from elsewhere: an id outside [0, experts) has no row, and position -1.
+ *
+ * pmlb_route_grad: dlogits (the logits' type and row stride) from the weights' gradient (f32), at the same choice; an id
+ * outside [0, experts) takes no part.  An expert is chosen once by a token.  The choice itself and the bias have none. */
+#define PMLB_ROUTE_SOFTMAX 0
+#define PMLB_ROUTE_SIGMOID 1
+
+typedef struct {
+  int32_t dtype;
+  int32_t tokens, experts, top_k;
+  int32_t score;                     /* PMLB_ROUTE_* */
+  int32_t groups, top_groups;
+  int32_t renormalise;
+  double scale;
+  int64_t ld;                        /* elements between rows of logits (and of their gradient) */
+  int32_t rows, align;
+} pmlb_route_desc;
+
+pmlb_status pmlb_route_dispatch(const pmlb_route_desc* desc, pmlb_plan** plan);
+pmlb_status pmlb_route_invoke(pmlb_plan* plan, void* stream, const void* logits, const float* bias, float* weights,
+                              int32_t* ids, int32_t* offsets, int32_t* source, int32_t* position);
+pmlb_status pmlb_route_order(pmlb_plan* plan, void* stream, const int32_t* ids, int32_t* offsets, int32_t* source,
+                             int32_t* position);
+pmlb_status pmlb_route_grad(pmlb_plan* plan, void* stream, const void* logits, const int32_t* ids, const float* dweights,
+                            void* dlogits);
+
+/* ---------------------------------------------------------------- combination of the experts' rows
+ * (no counterpart in the reference)
+ *
+ *   out[t] = sum_j weights[t, j] * y[position[t, j]]     in the order of j, in f32, rounded once
+ * y [rows][width] and out [tokens][width] of one type (F32, BF16 or F16), weights f32 (NULL: ones, which is the gradient
+ * of gathering rows), position int32; a position outside [0, rows) is left out of the sum.
+ * Gradients:  dy[position[t, j]] = weights[t, j] * dout[t], zeros in the rows r of which source[r] is outside
+ * [0, tokens * top_k) (position and source are those of one routing, so that every row is written once);
+ * dweights[t, j] = sum over the width of dout[t] * y[position[t, j]], 0 for a position left out.
+ * Either may be NULL, and then only the other is computed. */
+typedef struct {
+  int32_t dtype;
+  int32_t tokens, top_k, width, rows;
+  int32_t reserved0;
+  int64_t ldy, ldo;                  /* elements between rows of y (and dy) and of out (and dout) */
+} pmlb_combine_desc;
+
+pmlb_status pmlb_combine_dispatch(const pmlb_combine_desc* desc, pmlb_plan** plan);
+pmlb_status pmlb_combine_invoke(pmlb_plan* plan, void* stream, const void* y, const float* weights,
+                                const int32_t* position, void* out);
+pmlb_status pmlb_combine_grad(pmlb_plan* plan, void* stream, const void* dout, const void* y, const float* weights,
+                              const int32_t* position, const int32_t* source, void* dy, float* dweights);
 
 #ifdef __cplusplus
 }

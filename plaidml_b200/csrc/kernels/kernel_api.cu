@@ -8,12 +8,16 @@
 #include <new>
 #include <string>
 
+#include "block_gemm.h"
+#include "combine.h"
 #include "contract_route.h"
 #include "f32_mma.h"
 #include "generic.h"
 #include "pmlb_kernels.h"
 #include "prepass.h"
+#include "quant.h"
 #include "reduce.h"
+#include "route.h"
 #include "s2d_pool.h"
 #include "special.h"
 #include "tc_gemm.cuh"
@@ -83,7 +87,8 @@ bool have_sm100(std::string* why) {
 // launches logs its pipeline timeline to.
 long long* g_trace_buffer = nullptr;
 
-enum PlanKind { kPlanGemm, kPlanConv, kPlanReduce, kPlanPool, kPlanContract, kPlanEltwise, kPlanSpecial };
+enum PlanKind { kPlanGemm, kPlanConv, kPlanReduce, kPlanPool, kPlanContract, kPlanEltwise, kPlanSpecial,
+                kPlanBlockGemm, kPlanQuant, kPlanRoute, kPlanCombine };
 
 }  // namespace
 
@@ -122,6 +127,10 @@ struct pmlb_plan {
   pmlb::ProductForm product;     // contraction on the tensor cores (f32_mma)
   pmlb::EltwiseParams eltwise;
   pmlb_special_desc special;
+  pmlb_block_gemm_desc block_gemm;
+  pmlb_quant_desc quant;
+  pmlb_route_desc route;
+  pmlb_combine_desc combine;
 };
 
 namespace {
@@ -1494,6 +1503,293 @@ pmlb_status pmlb_special_invoke(pmlb_plan* plan, void* stream_, const void* in0,
   }
   if (e != cudaSuccess) return cuda_fail(e, "gather / scatter / argsort / prng launch");
   return PMLB_OK;
+}
+
+// ------------------------------------------------------------------ products of 8-bit floats, quantisation, routing, combination
+
+namespace {
+
+bool is_f8(int dtype) { return dtype == PMLB_F8E4M3 || dtype == PMLB_F8E5M2; }
+bool is_f32_or_16(int dtype) { return dtype == PMLB_F32 || dtype == PMLB_BF16 || dtype == PMLB_F16; }
+bool on_bytes(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// The device that the plan was made on, for the duration of a call from a thread that has another one current.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    cudaGetDevice(&before_);
+    if (before_ != device) cudaSetDevice(device), changed_ = true;
+  }
+  ~OnDevice() {
+    if (changed_) cudaSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+};
+
+std::string block_gemm_problem(const pmlb_block_gemm_desc& d) {
+  if (!is_f8(d.a_dtype) || !is_f8(d.b_dtype)) return "block_gemm: operands are 8-bit floats";
+  if (!is_f32_or_16(d.out_dtype)) return "block_gemm: the result is f32, bf16 or f16";
+  if (d.m < 0 || d.n <= 0 || d.k <= 0) return "block_gemm: n and k must be positive, m not negative";
+  // (tile coordinates and rounded-up lengths stay in 32 bits)
+  if (d.m > (1 << 30) || d.n > (1 << 30) || d.k > (1 << 30)) return "block_gemm: sizes above 2^30";
+  if (d.groups < 0 || d.groups > 1024) return "block_gemm: groups must be 0..1024";
+  if (d.groups > 0 && d.group_dim != PMLB_GROUP_ROWS && d.group_dim != PMLB_GROUP_TERMS) return "block_gemm: unknown group dimension";
+  if (d.b_scale_rows != 128 && d.b_scale_rows != 1) return "block_gemm: B has a scale for each 128 rows or for each row";
+  if (d.lda < d.k || d.ldb < d.k || d.ldc < d.n) return "block_gemm: a row stride smaller than a row";
+  if (d.lda % 16 != 0 || d.ldb % 16 != 0) return "block_gemm: lda and ldb must be multiples of 16";
+  // (a tensor map's strides are below 2^40 bytes)
+  if (d.lda >= (1LL << 40) || d.ldb >= (1LL << 40) || d.ldc >= (1LL << 40)) return "block_gemm: row strides of 2^40 and more";
+  if (d.groups > 0) {
+    const bool by_rows = d.group_dim == PMLB_GROUP_ROWS;
+    if (by_rows && (d.stride_b % 16 != 0 || d.stride_b < 0 || d.stride_b >= (1LL << 40))) {
+      return "block_gemm: stride_b must be a multiple of 16, not negative and below 2^40";
+    }
+    if (by_rows && d.stride_b < (d.n - 1) * d.ldb + d.k && d.stride_b != 0) return "block_gemm: the groups' B overlap";
+    if (!by_rows && d.stride_c < (d.m - 1) * d.ldc + d.n && d.groups > 1 && d.m > 0) return "block_gemm: the groups' C overlap";
+  }
+  if (d.a_scale_row < 0 || d.a_scale_block < 0 || d.b_scale_row < 0 || d.b_scale_block < 0 || d.b_scale_group < 0) {
+    return "block_gemm: negative stride of scales";
+  }
+  return "";
+}
+
+std::string quant_problem(const pmlb_quant_desc& d) {
+  if (!is_f32_or_16(d.in_dtype)) return "quant: the input is f32, bf16 or f16";
+  if (!is_f8(d.out_dtype)) return "quant: the result is an 8-bit float type";
+  if (d.form < PMLB_QUANT_ROWS || d.form > PMLB_QUANT_TILES_TRANSPOSED) return "quant: unknown form";
+  if (d.rows < 0 || d.cols <= 0 || d.batch <= 0) return "quant: cols and batch must be positive, rows not negative";
+  const bool turned = d.form == PMLB_QUANT_COLUMNS || d.form == PMLB_QUANT_TILES_TRANSPOSED;
+  if (d.ldx < d.cols || d.ldq < (turned ? d.rows : d.cols)) return "quant: a row stride smaller than a row";
+  if (d.rows > (1 << 30) || d.cols > (1 << 30)) return "quant: sizes above 2^30";
+  if (d.batch > 65535 || (d.form != PMLB_QUANT_ROWS && (d.rows + 127) / 128 > 65535)) return "quant: more rows or batch entries than one launch takes";
+  if (d.form == PMLB_QUANT_ROWS && ((d.cols + 511LL) / 512 * d.rows + 7) / 8 > 0x7fffffffLL) return "quant: more rows than one launch takes";
+  if (d.scale_row < 0 || d.scale_block < 0 || (d.batch > 1 && (d.stride_x < 0 || d.stride_q < 0 || d.stride_scale < 0))) return "quant: negative stride";
+  if (d.source_rows < 0) return "quant: negative source_rows";
+  if (d.source_rows > 0 && (d.form != PMLB_QUANT_ROWS || d.batch != 1)) return "quant: rows are taken by index in the form of rows, batch 1";
+  if (d.source_rows > 0 && d.source_div <= 0) return "quant: source_div must be positive";
+  return "";
+}
+
+std::string route_problem(const pmlb_route_desc& d) {
+  if (!is_f32_or_16(d.dtype)) return "route: the logits are f32, bf16 or f16";
+  if (d.tokens < 0 || d.experts <= 0 || d.top_k <= 0) return "route: experts and top_k must be positive, tokens not negative";
+  if (d.experts > 1024 || d.top_k > 32 || d.groups > 32) return "route: at most 1024 experts, 32 choices and 32 groups";
+  if (d.score != PMLB_ROUTE_SOFTMAX && d.score != PMLB_ROUTE_SIGMOID) return "route: unknown score";
+  if (d.groups <= 0 || d.experts % d.groups != 0) return "route: groups must divide the experts";
+  if (d.top_groups <= 0 || d.top_groups > d.groups) return "route: top_groups must be 1..groups";
+  if (d.top_k > d.experts / d.groups * d.top_groups) return "route: more choices than experts to choose from";
+  if (d.ld < d.experts) return "route: a row stride smaller than a row";
+  if (!(d.scale - d.scale == 0.0)) return "route: scale is not finite";
+  const long long pairs = static_cast<long long>(d.tokens) * d.top_k;
+  if (pairs > (1 << 24)) return "route: more than 2^24 pairs";
+  if (d.rows < 0 || (d.rows > 0 && (d.align < 1 || d.align > 1024))) return "route: rows must not be negative, align 1..1024";
+  if (d.rows > 0) {
+    const long long most = pairs + std::min<long long>(d.experts, pairs) * (d.align - 1);
+    if (d.rows < most / d.align * d.align) return "route: fewer rows than the experts' segments may need";
+  }
+  return "";
+}
+
+std::string combine_problem(const pmlb_combine_desc& d) {
+  if (!is_f32_or_16(d.dtype)) return "combine: rows are f32, bf16 or f16";
+  if (d.tokens < 0 || d.top_k <= 0 || d.width <= 0 || d.rows < 0) return "combine: top_k and width must be positive, tokens and rows not negative";
+  if (d.ldy < d.width || d.ldo < d.width) return "combine: a row stride smaller than a row";
+  if (static_cast<long long>(d.tokens) * d.top_k > (1 << 30) || d.rows > (1 << 30) || d.width > (1 << 30)) return "combine: sizes above 2^30";
+  return "";
+}
+
+pmlb_plan* new_plan(PlanKind kind, const char* name) {
+  pmlb_plan* plan = new (std::nothrow) pmlb_plan();
+  if (!plan) return nullptr;
+  plan->kind = kind;
+  plan->kind_name = name;
+  cudaGetDevice(&plan->device);
+  return plan;
+}
+
+}  // namespace
+
+pmlb_status pmlb_block_gemm_dispatch(const pmlb_block_gemm_desc* d, pmlb_plan** out) {
+  if (!d || !out) return fail(PMLB_ERR_INVALID, "null argument");
+  *out = nullptr;
+  const std::string problem = block_gemm_problem(*d);
+  if (!problem.empty()) return fail(PMLB_ERR_INVALID, problem);
+  std::string why;
+  if (!have_sm100(&why)) return fail(PMLB_ERR_UNSUPPORTED, why);
+  pmlb_plan* plan = new_plan(kPlanBlockGemm, "block_gemm");
+  if (!plan) return fail(PMLB_ERR_INVALID, "out of host memory");
+  plan->block_gemm = *d;
+  plan->status = pmlb::f32_mma_status_word();   // (the library's own word: plans hold no device memory)
+  plan->owns_status = false;
+  if (!plan->status) {
+    pmlb_plan_free(plan);
+    return fail(PMLB_ERR_CUDA, "block_gemm: no status word");
+  }
+  *out = plan;
+  return PMLB_OK;
+}
+
+pmlb_status pmlb_block_gemm_invoke(pmlb_plan* plan, void* stream, const void* a, const float* a_scale, const void* b,
+                                   const float* b_scale, const int32_t* offsets, void* c) {
+  if (!plan || plan->kind != kPlanBlockGemm) return fail(PMLB_ERR_INVALID, "not a block_gemm plan");
+  const pmlb_block_gemm_desc& d = plan->block_gemm;
+  if (d.m == 0) return PMLB_OK;
+  if (!a || !a_scale || !b || !b_scale || !c) return fail(PMLB_ERR_INVALID, "block_gemm: null operand");
+  if ((d.groups > 0) != (offsets != nullptr)) return fail(PMLB_ERR_INVALID, "block_gemm: offsets go with groups");
+  if (!on_bytes(a, 16) || !on_bytes(b, 16)) return fail(PMLB_ERR_INVALID, "block_gemm: operands must start on 16 bytes");
+  if (!on_bytes(a_scale, 4) || !on_bytes(b_scale, 4) || !on_bytes(offsets, 4) || !on_bytes(c, d.out_dtype == PMLB_F32 ? 4 : 2)) {
+    return fail(PMLB_ERR_INVALID, "block_gemm: a pointer that is not aligned to its elements");
+  }
+  OnDevice on(plan->device);
+  std::string err;
+  const int st = pmlb::block_gemm_launch(d, a, a_scale, b, b_scale, offsets, c, plan->status, static_cast<cudaStream_t>(stream), &err);
+  return st == 0 ? PMLB_OK : fail(static_cast<pmlb_status>(st), err);
+}
+
+pmlb_status pmlb_quant_dispatch(const pmlb_quant_desc* d, pmlb_plan** out) {
+  if (!d || !out) return fail(PMLB_ERR_INVALID, "null argument");
+  *out = nullptr;
+  const std::string problem = quant_problem(*d);
+  if (!problem.empty()) return fail(PMLB_ERR_INVALID, problem);
+  std::string why;
+  if (!have_sm100(&why)) return fail(PMLB_ERR_UNSUPPORTED, why);
+  static const char* const names[] = {"quant_rows", "quant_columns", "quant_tiles", "quant_tiles_transposed"};
+  pmlb_plan* plan = new_plan(kPlanQuant, names[d->form]);
+  if (!plan) return fail(PMLB_ERR_INVALID, "out of host memory");
+  plan->quant = *d;
+  *out = plan;
+  return PMLB_OK;
+}
+
+pmlb_status pmlb_quant_invoke(pmlb_plan* plan, void* stream, const void* x, const int32_t* rows, void* q, float* scale) {
+  if (!plan || plan->kind != kPlanQuant) return fail(PMLB_ERR_INVALID, "not a quant plan");
+  const pmlb_quant_desc& d = plan->quant;
+  if (d.rows == 0) return PMLB_OK;
+  if (!x || !q || !scale) return fail(PMLB_ERR_INVALID, "quant: null tensor");
+  if ((d.source_rows > 0) != (rows != nullptr)) return fail(PMLB_ERR_INVALID, "quant: rows go with source_rows");
+  if (!on_bytes(x, d.in_dtype == PMLB_F32 ? 4 : 2) || !on_bytes(scale, 4) || !on_bytes(rows, 4)) {
+    return fail(PMLB_ERR_INVALID, "quant: a pointer that is not aligned to its elements");
+  }
+  OnDevice on(plan->device);
+  const cudaError_t e = pmlb::launch_quant(d, x, rows, q, scale, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PMLB_OK : cuda_fail(e, "quant launch");
+}
+
+pmlb_status pmlb_route_dispatch(const pmlb_route_desc* d, pmlb_plan** out) {
+  if (!d || !out) return fail(PMLB_ERR_INVALID, "null argument");
+  *out = nullptr;
+  const std::string problem = route_problem(*d);
+  if (!problem.empty()) return fail(PMLB_ERR_INVALID, problem);
+  std::string why;
+  if (!have_sm100(&why)) return fail(PMLB_ERR_UNSUPPORTED, why);
+  pmlb_plan* plan = new_plan(kPlanRoute, "route");
+  if (!plan) return fail(PMLB_ERR_INVALID, "out of host memory");
+  plan->route = *d;
+  *out = plan;
+  return PMLB_OK;
+}
+
+pmlb_status pmlb_route_order(pmlb_plan* plan, void* stream, const int32_t* ids, int32_t* offsets, int32_t* source,
+                             int32_t* position) {
+  if (!plan || plan->kind != kPlanRoute) return fail(PMLB_ERR_INVALID, "not a route plan");
+  const pmlb_route_desc& d = plan->route;
+  if (d.rows == 0 && d.tokens > 0) return fail(PMLB_ERR_INVALID, "route: a plan without rows gives no order");
+  if (!offsets || (d.tokens > 0 && (!ids || !position)) || (d.rows > 0 && !source)) return fail(PMLB_ERR_INVALID, "route: null tensor");
+  if (!on_bytes(ids, 4) || !on_bytes(offsets, 4) || !on_bytes(source, 4) || !on_bytes(position, 4)) {
+    return fail(PMLB_ERR_INVALID, "route: a pointer that is not aligned to its elements");
+  }
+  OnDevice on(plan->device);
+  const cudaError_t e = pmlb::launch_route_order(d, ids, offsets, source, position, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PMLB_OK : cuda_fail(e, "route order launch");
+}
+
+pmlb_status pmlb_route_invoke(pmlb_plan* plan, void* stream, const void* logits, const float* bias, float* weights,
+                              int32_t* ids, int32_t* offsets, int32_t* source, int32_t* position) {
+  if (!plan || plan->kind != kPlanRoute) return fail(PMLB_ERR_INVALID, "not a route plan");
+  const pmlb_route_desc& d = plan->route;
+  if (d.tokens > 0 && (!logits || !weights || !ids)) return fail(PMLB_ERR_INVALID, "route: null tensor");
+  if (d.rows > 0 && (!offsets || !source || (d.tokens > 0 && !position))) return fail(PMLB_ERR_INVALID, "route: null tensor of the order");
+  if (!on_bytes(logits, d.dtype == PMLB_F32 ? 4 : 2) || !on_bytes(bias, 4) || !on_bytes(weights, 4) || !on_bytes(ids, 4) ||
+      !on_bytes(offsets, 4) || !on_bytes(source, 4) || !on_bytes(position, 4)) {
+    return fail(PMLB_ERR_INVALID, "route: a pointer that is not aligned to its elements");
+  }
+  OnDevice on(plan->device);
+  if (d.tokens > 0) {
+    const cudaError_t e = pmlb::launch_route(d, logits, bias, weights, ids, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "route launch");
+  }
+  if (d.rows > 0) {
+    const cudaError_t e = pmlb::launch_route_order(d, ids, offsets, source, position, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "route order launch");
+  }
+  return PMLB_OK;
+}
+
+pmlb_status pmlb_route_grad(pmlb_plan* plan, void* stream, const void* logits, const int32_t* ids, const float* dweights,
+                            void* dlogits) {
+  if (!plan || plan->kind != kPlanRoute) return fail(PMLB_ERR_INVALID, "not a route plan");
+  const pmlb_route_desc& d = plan->route;
+  if (d.tokens == 0) return PMLB_OK;
+  if (!logits || !ids || !dweights || !dlogits) return fail(PMLB_ERR_INVALID, "route: null tensor");
+  const size_t eb = d.dtype == PMLB_F32 ? 4 : 2;
+  if (!on_bytes(logits, eb) || !on_bytes(dlogits, eb) || !on_bytes(ids, 4) || !on_bytes(dweights, 4)) {
+    return fail(PMLB_ERR_INVALID, "route: a pointer that is not aligned to its elements");
+  }
+  OnDevice on(plan->device);
+  const cudaError_t e = pmlb::launch_route_grad(d, logits, ids, dweights, dlogits, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PMLB_OK : cuda_fail(e, "route gradient launch");
+}
+
+pmlb_status pmlb_combine_dispatch(const pmlb_combine_desc* d, pmlb_plan** out) {
+  if (!d || !out) return fail(PMLB_ERR_INVALID, "null argument");
+  *out = nullptr;
+  const std::string problem = combine_problem(*d);
+  if (!problem.empty()) return fail(PMLB_ERR_INVALID, problem);
+  std::string why;
+  if (!have_sm100(&why)) return fail(PMLB_ERR_UNSUPPORTED, why);
+  pmlb_plan* plan = new_plan(kPlanCombine, "combine");
+  if (!plan) return fail(PMLB_ERR_INVALID, "out of host memory");
+  plan->combine = *d;
+  *out = plan;
+  return PMLB_OK;
+}
+
+pmlb_status pmlb_combine_invoke(pmlb_plan* plan, void* stream, const void* y, const float* weights,
+                                const int32_t* position, void* out) {
+  if (!plan || plan->kind != kPlanCombine) return fail(PMLB_ERR_INVALID, "not a combine plan");
+  const pmlb_combine_desc& d = plan->combine;
+  if (d.tokens == 0) return PMLB_OK;
+  if ((!y && d.rows > 0) || !position || !out) return fail(PMLB_ERR_INVALID, "combine: null tensor");
+  const size_t eb = d.dtype == PMLB_F32 ? 4 : 2;
+  if (!on_bytes(y, eb) || !on_bytes(out, eb) || !on_bytes(weights, 4) || !on_bytes(position, 4)) {
+    return fail(PMLB_ERR_INVALID, "combine: a pointer that is not aligned to its elements");
+  }
+  OnDevice on(plan->device);
+  const cudaError_t e = pmlb::launch_combine(d, y, weights, position, out, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PMLB_OK : cuda_fail(e, "combine launch");
+}
+
+pmlb_status pmlb_combine_grad(pmlb_plan* plan, void* stream, const void* dout, const void* y, const float* weights,
+                              const int32_t* position, const int32_t* source, void* dy, float* dweights) {
+  if (!plan || plan->kind != kPlanCombine) return fail(PMLB_ERR_INVALID, "not a combine plan");
+  const pmlb_combine_desc& d = plan->combine;
+  if (d.rows == 0) dy = nullptr;
+  if (d.tokens == 0) dweights = nullptr;
+  if (!dy && !dweights) return d.rows == 0 || d.tokens == 0 ? PMLB_OK : fail(PMLB_ERR_INVALID, "combine: no gradient asked for");
+  if ((d.tokens > 0 && (!dout || !position)) || (dy && !source) || (dweights && !y && d.rows > 0)) return fail(PMLB_ERR_INVALID, "combine: null tensor");
+  const size_t eb = d.dtype == PMLB_F32 ? 4 : 2;
+  if (!on_bytes(dout, eb) || !on_bytes(y, eb) || !on_bytes(dy, eb) || !on_bytes(weights, 4) || !on_bytes(position, 4) || !on_bytes(source, 4) ||
+      !on_bytes(dweights, 4)) {
+    return fail(PMLB_ERR_INVALID, "combine: a pointer that is not aligned to its elements");
+  }
+  OnDevice on(plan->device);
+  const cudaError_t e = pmlb::launch_combine_grad(d, dout, y, weights, position, source, dy, dweights, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? PMLB_OK : cuda_fail(e, "combine gradient launch");
 }
 
 }  // extern "C"

@@ -462,7 +462,7 @@ __device__ __forceinline__ void st_global_v8(void* ptr, const uint4& lo, const u
                : "memory");
 }
 
-enum : int { kMmaF16 = 0, kMmaTf32 = 1, kMmaI8 = 2 };
+enum : int { kMmaF16 = 0, kMmaTf32 = 1, kMmaI8 = 2, kMmaF8 = 3 };
 
 // D[tmem] (+)= A[smem] * B[smem]; `accumulate` == 0 overwrites D.
 template <int KIND>
@@ -484,6 +484,16 @@ __device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t a_desc, uint64_
         ".reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else if constexpr (KIND == kMmaF8) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
         "}\n"
         :
         : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
@@ -523,6 +533,16 @@ __device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, ui
         ".reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else if constexpr (KIND == kMmaF8) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
         "}\n"
         :
         : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
@@ -581,6 +601,8 @@ __device__ __forceinline__ void tc_mma_x4(uint32_t d_tmem, uint32_t a_lo, uint32
       PMLB_MMA_X4("tcgen05.mma.cta_group::2.kind::f16");
     } else if constexpr (KIND == kMmaTf32) {
       PMLB_MMA_X4("tcgen05.mma.cta_group::2.kind::tf32");
+    } else if constexpr (KIND == kMmaF8) {
+      PMLB_MMA_X4("tcgen05.mma.cta_group::2.kind::f8f6f4");
     } else {
       PMLB_MMA_X4("tcgen05.mma.cta_group::2.kind::i8");
     }
@@ -589,6 +611,8 @@ __device__ __forceinline__ void tc_mma_x4(uint32_t d_tmem, uint32_t a_lo, uint32
       PMLB_MMA_X4("tcgen05.mma.cta_group::1.kind::f16");
     } else if constexpr (KIND == kMmaTf32) {
       PMLB_MMA_X4("tcgen05.mma.cta_group::1.kind::tf32");
+    } else if constexpr (KIND == kMmaF8) {
+      PMLB_MMA_X4("tcgen05.mma.cta_group::1.kind::f8f6f4");
     } else {
       PMLB_MMA_X4("tcgen05.mma.cta_group::1.kind::i8");
     }

@@ -184,6 +184,13 @@ bool tc_supported(std::string* why) {
   return true;
 }
 
+bool tc_encode_bytes(void* map, const void* base, long long d0, long long d1, long long d2, long long stride1, long long stride2, int rows,
+                     std::string* err) {
+  if (!tc_supported(err)) return false;
+  return encode3d(static_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, d0, d1, d2, stride1, stride2, 128,
+                  static_cast<uint32_t>(rows), 1, err);
+}
+
 int tc_launch(const TcLaunch& L, cudaStream_t stream, std::string* err) {
   load_driver_entry_points();
   if (!g_encode_tiled || !g_encode_im2col) {

@@ -26,25 +26,37 @@ namespace {
 
 constexpr int kBlock = 128;       // terms per scale, and rows of B per scale
 constexpr int kMaxGroups = 1024;
-constexpr int kSumWarps = 8;
-constexpr int kThreads = 128 + kSumWarps * 32;   // warp 0 loads, warp 1 issues MMAs, warps 4..11 add
-constexpr int kLoaderRegs = 56, kSumRegs = 224;  // (128 * 56 + 256 * 224 = 384 * 168, what the block is launched with)
+
+// Which scales differ within a warp's part of an accumulator (32 rows, half of the columns).
+enum Scales { kOfRows, kOfBoth };
 
 // BN: columns of the accumulators.  SWAP: their rows are rows of B (weights) and their columns rows of A (tokens), for products
 // of few tokens: the 128 rows of an MMA are then all of use, and BN need only be as large as there are tokens.
-// VEC: each column has a scale of its own (else the tile's 128 columns of a warp share one).
-template <int BN_, bool SWAP_, bool VEC_>
+// CTAS = 2: a cluster of two CTAs on one tile of 256 rows, each with 128 of them and half of the other operand.
+template <int BN_, bool SWAP_, Scales SCALES_, int CTAS_ = 1>
 struct BlockCfg {
-  static constexpr int BN = BN_;
-  static constexpr bool kSwap = SWAP_, kVec = VEC_;
-  static constexpr int kTileP = 128 * 128, kTileQ = BN * 128;
+  static constexpr int BN = BN_, CTAS = CTAS_;
+  static constexpr bool kSwap = SWAP_;
+  static constexpr Scales kScales = SCALES_;
+  static constexpr int kSumWarps = 8;
+  static constexpr int kThreads = 128 + kSumWarps * 32;   // warp 0 loads, warp 1 issues MMAs, warps 4 and up add
+  static constexpr int kLoaderRegs = 56, kSumRegs = 224;  // (128 * 56 + 256 * 224 = 384 * 168, what the block is launched with)
+  static constexpr int kCols = BN / (kSumWarps / 4);       // columns that a warp adds
+  static constexpr int kTileP = 128 * 128, kTileQ = BN / CTAS * 128;
   static constexpr int kStageBytes = kTileP + kTileQ;
   static constexpr int kAccs = BN == 256 ? 2 : 4;
   static constexpr int kTmemCols = kAccs * BN;
-  static constexpr int kPartBytes = kSwap ? BN * 128 * 4 : 0;                       // this CTA's sums, where K is split
-  static constexpr int kTailBytes = 512 + 3 * (kMaxGroups + 4) * 4;
-  static constexpr int kStages = std::min(10, (231000 - 1024 - kPartBytes - kTailBytes) / kStageBytes);
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kPartBytes + kTailBytes;
+  static constexpr bool kSplits = kSwap && CTAS == 1;                               // K may be shared by a cluster
+  static constexpr int kPartBytes = kSplits ? BN * 128 * 4 : 0;                     // this CTA's sums, where it is
+  // Scales of a block: one for each row of the accumulator, then one for each column (or for each 128 of them); kAhead blocks are
+  // on their way (see the warp that fetches them for what bounds it).
+  static constexpr int kSlots = kScales == kOfBoth && BN == 256 ? 8 : 16, kAhead = kSlots - 2 * kAccs - 1;
+  static constexpr int kSlotFloats = 128 + (kScales == kOfBoth ? BN : 4);
+  static constexpr int kScaleBytes = kSlots * kSlotFloats * 4;
+  static constexpr int kStageOutBytes = kSwap ? 0 : kSumWarps * 8192;    // results on their way out: two boxes of 32 rows of 128 bytes per warp
+  static constexpr int kTailBytes = 512 + 2 * (kMaxGroups + 4) * 4;
+  static constexpr int kStages = std::min(10, (232448 - 1024 - kPartBytes - kScaleBytes - kStageOutBytes - kTailBytes) / kStageBytes);
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kPartBytes + kScaleBytes + kStageOutBytes + kTailBytes;
   static_assert(kStages >= 3 && kSmem <= 232448, "shared memory");
 };
 
@@ -79,35 +91,65 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
   return make_float2(__uint_as_float(lo), __uint_as_float(hi));
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+// c += a * b.  (volatile: stays behind the wait for the TMEM loads whose registers it reads)
+__device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) { asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b)); }
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 
+#define PMLB_OUT_8(i) \
+  "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[N]) {
-  if constexpr (N == 32) {
+  if constexpr (N == 64) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, "
+        "%45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+        : PMLB_OUT_8(0), PMLB_OUT_8(8), PMLB_OUT_8(16), PMLB_OUT_8(24), PMLB_OUT_8(32), PMLB_OUT_8(40), PMLB_OUT_8(48), PMLB_OUT_8(56)
+        : "r"(taddr)
+        : "memory");
+  } else if constexpr (N == 32) {
     tmem_ld_32x32(taddr, v);
   } else if constexpr (N == 16) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : PMLB_OUT_8(0), PMLB_OUT_8(8)
         : "r"(taddr)
         : "memory");
   } else {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : PMLB_OUT_8(0)
                  : "r"(taddr)
                  : "memory");
   }
 }
 
+#undef PMLB_OUT_8
+
 __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
   return v;
+}
+
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four bytes from global to shared memory without a register; groups of them complete in order.
+__device__ __forceinline__ void copy_async_4(uint32_t to, const float* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // All threads of the cluster, from code where the warp's lanes may have parted.
@@ -125,44 +167,59 @@ __device__ __forceinline__ void store_one(const BlockGemmParams& p, long long at
   }
 }
 
-// Eight consecutive columns of a row from element `at` on, `n` of which exist.
-__device__ __forceinline__ void store_eight(const BlockGemmParams& p, long long at, const float (&v)[8], int n) {
-  if (n >= 8 && p.out_align >= 16) {
-    if (p.out_dtype == PMLB_F32) {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint4 u;
-      if (p.out_dtype == PMLB_BF16) {
-        u = make_uint4(cvt_pack16<true, false>(v[0], v[1]), cvt_pack16<true, false>(v[2], v[3]), cvt_pack16<true, false>(v[4], v[5]),
-                       cvt_pack16<true, false>(v[6], v[7]));
-      } else {
-        u = make_uint4(cvt_pack16<false, false>(v[0], v[1]), cvt_pack16<false, false>(v[2], v[3]), cvt_pack16<false, false>(v[4], v[5]),
-                       cvt_pack16<false, false>(v[6], v[7]));
-      }
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at) = u;
+// Results leave through shared memory in boxes of 32 rows of 128 bytes (64 columns of 16 bits, or 32 of 32 bits), in the layout
+// of a TMA store with 128-byte swizzle: 16-byte pieces permuted by the row, which spreads a lane's row over the banks.
+__device__ __forceinline__ uint32_t box_piece(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }
+
+// A box by plain stores: rows [0, rows) of C from element `base` on, `n` columns of which exist.
+__device__ __forceinline__ void store_box(const BlockGemmParams& p, uint32_t at, long long base, int rows, int n, int lane) {
+  const int bytes = p.out_dtype == PMLB_F32 ? 4 : 2;
+  char* dst = static_cast<char*>(p.out) + base * bytes;
+  const long long step = p.ldc * bytes;
+  if (n * bytes >= 128 && p.out_align >= 16) {
+    const int piece = lane & 7;
+#pragma unroll 4
+    for (int r = lane >> 3; r < 32; r += 4) {
+      const uint4 u = ld_shared_v4(at + box_piece(r, piece));
+      if (r < rows) *reinterpret_cast<uint4*>(dst + r * step + piece * 16) = u;
+    }
+  } else if (bytes == 4) {
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      const float v = ld_shared_f32(at + box_piece(r, lane >> 2) + (lane & 3) * 4);
+      if (lane < n) *reinterpret_cast<float*>(dst + r * step + lane * 4) = v;
     }
   } else {
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (e < n) store_one(p, at + e, v[e]);
+      for (int c = lane; c < 64; c += 32) {
+        uint16_t h;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + box_piece(r, c >> 3) + (c & 7) * 2) : "memory");
+        if (c < n) *reinterpret_cast<uint16_t*>(dst + r * step + c * 2) = h;
+      }
     }
   }
 }
 
 template <class Cfg>
-__global__ void __launch_bounds__(kThreads, 1)
-    block_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ BlockGemmParams p) {
+__global__ void __launch_bounds__(Cfg::kThreads, 1)
+    block_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_c,
+                      const __grid_constant__ BlockGemmParams p) {
   constexpr int BN = Cfg::BN, kStages = Cfg::kStages, kAccs = Cfg::kAccs;
-  constexpr bool SWAP = Cfg::kSwap, VEC = Cfg::kVec;
-  constexpr int kTileRows = SWAP ? BN : 128, kTileCols = SWAP ? 128 : BN;   // of C
+  constexpr int CTAS = Cfg::CTAS;
+  constexpr bool SWAP = Cfg::kSwap, PAIR = CTAS == 2;
+  constexpr Scales SCALES = Cfg::kScales;
+  constexpr int kTileRows = SWAP ? BN : 128 * CTAS, kTileCols = SWAP ? 128 * CTAS : BN;   // of C
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t ring = (raw + 1023u) & ~1023u;
   uint8_t* after_ring = smem_raw + (ring - raw) + kStages * Cfg::kStageBytes;
+  const uint32_t out_stage = smem_u32(after_ring);   // (1024-byte aligned, as the boxes' swizzle wants it)
+  after_ring += Cfg::kStageOutBytes;
   float* part = reinterpret_cast<float*>(after_ring);
-  uint8_t* tail = after_ring + Cfg::kPartBytes;
+  const uint32_t scale_ring = smem_u32(after_ring + Cfg::kPartBytes);
+  uint8_t* tail = after_ring + Cfg::kPartBytes + Cfg::kScaleBytes;
   const uint32_t bar0 = smem_u32(tail);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (10 + s); };
@@ -170,11 +227,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto tempty_bar = [&](int a) { return bar0 + 8u * (24 + a); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 264);   // flag, code, wait limit
-  int* begins = reinterpret_cast<int*>(tail + 512);         // groups of rows: first row,
-  int* ends = begins + kMaxGroups + 4;                      // row behind the last,
-  int* before = ends + kMaxGroups + 4;                      // row tiles of the groups before
+  int* begins = reinterpret_cast<int*>(tail + 512);         // groups of rows: first row (and, behind the last one, the end),
+  int* before = begins + kMaxGroups + 4;                    // row tiles of the groups before
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
+  const int side = PAIR ? static_cast<int>(cluster_ctarank()) : 0;   // CTA of the pair
 
   if (threadIdx.x == 64) {
     for (int s = 0; s < kStages; ++s) {
@@ -182,8 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < kAccs; ++a) {
-      mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), kSumWarps);
+      mbar_init(tfull_bar(a), 2);   // (the products, and their scales)
+      mbar_init(tempty_bar(a), Cfg::kSumWarps * CTAS);   // (pairs: both CTAs' warps, at the first CTA)
     }
     abort_flag[0] = 0;
     abort_flag[1] = 0;
@@ -192,9 +249,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (threadIdx.x == 96) {
     tma_prefetch_desc(&map_p);
     tma_prefetch_desc(&map_q);
+    if (!SWAP && p.out_align >= 16) tma_prefetch_desc(&map_c);
   } else if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), Cfg::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+      tmem_relinquish();
+    }
     tc_fence_before_sync();
   }
   grid_dependency_wait();
@@ -223,18 +286,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
       }
-      if (g < p.groups) begins[g] = lo, ends[g] = hi, before[g] = sum + x - tiles;
+      if (g < p.groups) begins[g] = lo, before[g] = sum + x - tiles;
       sum += __shfl_sync(0xffffffffu, x, 31);
     }
-    if (lane == 0) before[p.groups] = sum;
+    if (lane == 0) begins[p.groups] = top, before[p.groups] = sum;
   }
-  __syncthreads();
+  __syncwarp();
+  if constexpr (PAIR) {
+    cluster_sync_all();   // (the other CTA's barriers must exist before anything is sent to them)
+  } else {
+    __syncthreads();
+  }
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
 
-  const int units = static_cast<int>(gridDim.x) / p.split;
-  const int rank = static_cast<int>(blockIdx.x) % p.split;
-  const int first = static_cast<int>(blockIdx.x) / p.split;
+  const int share = PAIR ? 2 : p.split;   // CTAs of a tile
+  const int units = static_cast<int>(gridDim.x) / share;
+  const int rank = PAIR ? 0 : static_cast<int>(blockIdx.x) % share;
+  const int first = static_cast<int>(blockIdx.x) / share;
   const int per_group = p.tiles_m * p.tiles_n;
   const int total = p.groups == 0 ? per_group : (p.terms ? p.groups * per_group : before[p.groups] * p.tiles_n);
   // Every role walks the same tiles.
@@ -253,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nt = local / tiles;
       x.group = lo;
       x.row0 = begins[lo] + (local - nt * tiles) * kTileRows;
-      x.row_end = ends[lo];
+      x.row_end = begins[lo + 1];
       x.n0 = nt * kTileCols;
     } else {
       if (p.terms) {
@@ -282,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kLoaderRegs));
     if (warp == 0) {
       // ------------------------------------------------------------ loads
       const bool leader = elect_one();
@@ -291,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int t = first; t < total && ok; t += units) {
         const Tile x = tile_at(t);
-        const int py = SWAP ? x.n0 : x.row0, qy = SWAP ? x.row0 : x.n0;
+        const int py = (SWAP ? x.n0 : x.row0) + side * 128, qy = (SWAP ? x.row0 : x.n0) + side * (BN / CTAS);
         const int z = p.terms ? 0 : x.group;
         for (int kb = x.kb0; kb < x.kb1; ++kb) {
           if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag)) {
@@ -301,15 +370,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (leader) {
             const uint32_t s = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-            mbar_arrive_expect_tx(full_bar(stage), Cfg::kStageBytes);
-            tma_load_3d(s, &map_p, full_bar(stage), kb * kBlock, py, SWAP ? z : 0);
-            tma_load_3d(s + Cfg::kTileP, &map_q, full_bar(stage), kb * kBlock, qy, SWAP ? 0 : z);
+            if (side == 0) mbar_arrive_expect_tx(full_bar(stage), CTAS * Cfg::kStageBytes);
+            if constexpr (PAIR) {   // both CTAs' bytes are counted at the first one
+              const uint32_t fb = mapa_rank(full_bar(stage), 0);
+              tma_load_3d_pair(s, &map_p, fb, kb * kBlock, py, SWAP ? z : 0);
+              tma_load_3d_pair(s + Cfg::kTileP, &map_q, fb, kb * kBlock, qy, SWAP ? 0 : z);
+            } else {
+              tma_load_3d(s, &map_p, full_bar(stage), kb * kBlock, py, SWAP ? z : 0);
+              tma_load_3d(s + Cfg::kTileP, &map_q, full_bar(stage), kb * kBlock, qy, SWAP ? 0 : z);
+            }
           }
           __syncwarp();
           if (++stage == kStages) stage = 0, phase ^= 1u;
         }
       }
-    } else if (warp == 1) {
+    } else if (warp == 1 && side == 0) {
       // ------------------------------------------------------------ MMAs
       const bool leader = elect_one();
       const uint64_t desc0 = make_smem_desc_sw128(0, 16, 1024);
@@ -320,169 +395,290 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = first; t < total && ok; t += units) {
         const Tile x = tile_at(t);
         for (int kb = x.kb0; kb < x.kb1; ++kb) {
-          if (!mbar_wait_warp(tempty_bar(acc), acc_phase ^ 1u, abort_flag)) {
-            if (leader && abort_flag[1] == 0) abort_flag[1] = 2;
-            ok = false;
-            break;
-          }
+          // (the accumulator last: it is what the loop waits for)
           if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) {
             if (leader && abort_flag[1] == 0) abort_flag[1] = 3;
             ok = false;
             break;
           }
+          const uint32_t s = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+          const uint32_t lo_p = desc_lo | ((s & 0x3FFFFu) >> 4), lo_q = desc_lo | (((s + Cfg::kTileP) & 0x3FFFFu) >> 4);
+          if (!mbar_wait_warp(tempty_bar(acc), acc_phase ^ 1u, abort_flag)) {
+            if (leader && abort_flag[1] == 0) abort_flag[1] = 2;
+            ok = false;
+            break;
+          }
           tc_fence_after_sync();
           if (leader) {
-            const uint32_t s = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-            const uint32_t lo_p = desc_lo | ((s & 0x3FFFFu) >> 4), lo_q = desc_lo | (((s + Cfg::kTileP) & 0x3FFFFu) >> 4);
-            tc_mma_x4<kMmaF8, 1>(tmem_base + static_cast<uint32_t>(acc * BN), lo_p, lo_q, desc_hi, desc_hi, p.idesc, 0u, 2u, 2u);
-            tc_commit(empty_bar(stage));
-            tc_commit(tfull_bar(acc));
+            tc_mma_x4<kMmaF8, CTAS>(tmem_base + static_cast<uint32_t>(acc * BN), lo_p, lo_q, desc_hi, desc_hi, p.idesc, 0u, 2u, 2u);
+            if constexpr (PAIR) {
+              tc_commit_pair(tfull_bar(acc), 3);
+              tc_commit_pair(empty_bar(stage), 3);
+            } else {
+              tc_commit(tfull_bar(acc));
+              tc_commit(empty_bar(stage));
+            }
           }
           __syncwarp();
           if (++stage == kStages) stage = 0, phase ^= 1u;
           if (++acc == kAccs) acc = 0, acc_phase ^= 1u;
         }
       }
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ scales
+      // Asynchronous copies, kAhead blocks ahead and across tiles: fetched by the warps that use them, scales cost those a trip to
+      // L2 or HBM per block (78 us of a product of 4096^3 were then 15 us of waiting for scales).  A block's products are announced
+      // by the tensor core and by this warp.  Step s waits for the products of block s - kAccs: they were begun after all of block
+      // s - 2 kAccs had been read, so the slots up to block s - 2 kAccs - 1 are free.
+      constexpr int kRowCopies = 4, kColCopies = SCALES == kOfRows ? 1 : (BN + 31) / 32;
+      int ahead_t = first, ahead_kb = 0, ahead_end = 0, to = 0;
+      const float *row_from[kRowCopies], *col_from[kColCopies];
+      const long long row_step = SWAP ? p.bs_block : p.as_block, col_step = SWAP ? p.as_block : p.bs_block;
+      auto point_at = [&](int t) {   // the first block of tile t, or of the next one that has blocks
+        for (; t < total; t += units) {
+          const Tile x = tile_at(t);
+          if (x.kb0 == x.kb1) continue;
+          const float *sa = p.a_scale + x.kb0 * p.as_block, *sb = p.b_scale + (p.terms ? 0 : x.group) * p.bs_group + x.kb0 * p.bs_block;
+          auto of_token = [&](int i) { return sa + min(x.row0 + i, p.m - 1) * p.as_row; };
+          auto of_weight = [&](int i) { return sb + (min(x.n0 + i, p.n - 1) >> p.b_shift) * p.bs_row; };
+#pragma unroll
+          for (int e = 0; e < kRowCopies; ++e) {
+            const int i = side * 128 + e * 32 + lane;
+            row_from[e] = SWAP ? of_weight(i) : of_token(i);
+          }
+#pragma unroll
+          for (int e = 0; e < kColCopies; ++e) {
+            const int i = SCALES == kOfRows ? lane * 128 : e * 32 + lane;
+            col_from[e] = SWAP ? of_token(i) : of_weight(i);
+          }
+          ahead_kb = x.kb0, ahead_end = x.kb1;
+          break;
+        }
+        ahead_t = t;
+      };
+      auto request = [&]() {   // the next block's scales
+        if (ahead_t < total) {
+          const uint32_t at = scale_ring + static_cast<uint32_t>((to * Cfg::kSlotFloats + lane) * 4);
+#pragma unroll
+          for (int e = 0; e < kRowCopies; ++e) {
+            copy_async_4(at + e * 128, row_from[e]);
+            row_from[e] += row_step;
+          }
+#pragma unroll
+          for (int e = 0; e < kColCopies; ++e) {
+            if (SCALES == kOfRows ? lane < BN / 128 : e * 32 + lane < BN) copy_async_4(at + 512 + e * 128, col_from[e]);
+            col_from[e] += col_step;
+          }
+          if (++ahead_kb == ahead_end) point_at(ahead_t + units);
+        }
+        copy_async_commit();
+        if (++to == Cfg::kSlots) to = 0;
+      };
+      point_at(first);
+      for (int e = 0; e < Cfg::kAhead; ++e) request();
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      for (int t = first; t < total && ok; t += units) {
+        const Tile x = tile_at(t);
+        for (int kb = x.kb0; kb < x.kb1; ++kb) {
+          if (!mbar_wait_warp(tfull_bar(acc), acc_phase ^ 1u, abort_flag)) {
+            if (lane == 0 && abort_flag[1] == 0) abort_flag[1] = 5;
+            ok = false;
+            break;
+          }
+          request();
+          copy_async_wait<Cfg::kAhead>();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tfull_bar(acc));
+          if (++acc == kAccs) acc = 0, acc_phase ^= 1u;
+        }
+      }
+      copy_async_wait<0>();
     }
   } else {
     // ------------------------------------------------------------ sums
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSumRegs));
     const int w = warp - 4;
-    const int quarter = warp & 3, half = w >> 2;     // TMEM lanes [32 quarter, ...), columns [half * BN / 2, ...)
-    constexpr int kCols = BN / 2;
-    constexpr int kChunk = kCols < 32 ? kCols : 32;
-    constexpr int kMine = (kCols + 31) / 32;         // column scales that a lane fetches
-    const uint32_t t_mine = tmem_base + static_cast<uint32_t>(half * kCols) + (static_cast<uint32_t>(quarter * 32) << 16);
-    int acc = 0;
+    constexpr int kCols = Cfg::kCols;
+    const int quarter = warp & 3, first_col = (w >> 2) * kCols;   // TMEM lanes [32 quarter, ...), columns [first_col, ...)
+    // Columns loaded from TMEM at a time.  Two warps take turns on a scheduler, so one set of registers is enough; what counts is
+    // that the compiler finds them beside the sums without moving any (4096^3: 16 at a time 70 us, 32 76, 64 68; two sets
+    // of 32 73; a weight gradient's two scales per element: 100, 107, 120).
+    constexpr int kChunk = kCols < 16 ? kCols : (SCALES == kOfRows && kCols >= 64 ? 64 : 16), kChunks = kCols / kChunk;
+    const uint32_t t_mine = tmem_base + static_cast<uint32_t>(first_col) + (static_cast<uint32_t>(quarter * 32) << 16);
+    int acc = 0, slot = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
+    const uint32_t tempty_at_first = PAIR ? mapa_rank(tempty_bar(0), 0) : 0u;
+    // Waits for the accumulator's block and its scales; false: gave up.
+    auto ready = [&]() {
+      if (!mbar_wait_warp(tfull_bar(acc), acc_phase, abort_flag)) {
+        if (lane == 0 && abort_flag[1] == 0) abort_flag[1] = 4;
+        return false;
+      }
+      tc_fence_after_sync();
+      return true;
+    };
+    // Hands the accumulator back (all of it is in registers) and goes on to the next.
+    auto release = [&]() {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) {
+          mbar_arrive_cluster(tempty_at_first + 8u * acc);
+        } else {
+          mbar_arrive(tempty_bar(acc));
+        }
+      }
+      if (++acc == kAccs) acc = 0, acc_phase ^= 1u;
+    };
     for (int t = first; t < total && ok; t += units) {
       const Tile x = tile_at(t);
-      // scales of this thread's accumulator row, and of the columns
-      const int i = quarter * 32 + lane;
-      const int token = min(x.row0 + (SWAP ? 0 : i), p.m - 1), weight = min(x.n0 + (SWAP ? i : half * kCols), p.n - 1);
-      const float* sa = p.a_scale + (SWAP ? 0 : token * p.as_row);
-      const float* sb = p.b_scale + (p.terms ? 0 : x.group) * p.bs_group + (SWAP || !VEC ? (weight >> p.b_shift) * p.bs_row : 0);
-      const float* row_scale = SWAP ? sb : sa;
-      const float* col_scale = SWAP ? sa : sb;
-      const long long row_step = SWAP ? p.bs_block : p.as_block, col_step = SWAP ? p.as_block : p.bs_block;
-      long long col_at[kMine];
-      if constexpr (VEC) {
-#pragma unroll
-        for (int e = 0; e < kMine; ++e) {
-          const int j = half * kCols + e * 32 + min(lane, kCols - 1);
-          col_at[e] = SWAP ? min(x.row0 + j, p.m - 1) * p.as_row : min(x.n0 + j, p.n - 1) * p.bs_row;
-        }
-      } else {
-        col_at[0] = 0;
-      }
+      const int i = side * 128 + quarter * 32 + lane;   // the accumulator row of this thread
       uint64_t sum[kCols / 2];
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) sum[j] = 0;
-      float next_row = 0.f, next_col[kMine];
-      auto fetch = [&](int kb) {
-        next_row = __ldg(row_scale + kb * row_step);
-#pragma unroll
-        for (int e = 0; e < (VEC ? kMine : 1); ++e) next_col[e] = __ldg(col_scale + col_at[e] + kb * col_step);
+      float next_row = 0.f;    // the row's scale (kOfRows: times that of the columns) of the block that is ready
+      uint64_t row2 = 0;       // ... and of the one that is being added
+      uint32_t scales = 0;     // the columns' ones
+      auto read_scales = [&]() {
+        const uint32_t at = scale_ring + static_cast<uint32_t>(slot * Cfg::kSlotFloats * 4);
+        next_row = ld_shared_f32(at + (quarter * 32 + lane) * 4);
+        if constexpr (SCALES == kOfRows) next_row *= ld_shared_f32(at + 512u + (first_col / 128) * 4);
       };
-      if (x.kb0 < x.kb1) fetch(x.kb0);
-      for (int kb = x.kb0; kb < x.kb1; ++kb) {
-        const float rs = next_row;
-        float cs[kMine];
+      auto take_scales = [&]() {
+        row2 = pack2(next_row, next_row);
+        scales = scale_ring + static_cast<uint32_t>(slot * Cfg::kSlotFloats * 4) + 512u + first_col * 4;
+        if (++slot == Cfg::kSlots) slot = 0;
+      };
+      auto add = [&](uint32_t (&v)[kChunk], int c) {
 #pragma unroll
-        for (int e = 0; e < (VEC ? kMine : 1); ++e) cs[e] = next_col[e];
-        if (kb + 1 < x.kb1) fetch(kb + 1);
-        if (!mbar_wait_warp(tfull_bar(acc), acc_phase, abort_flag)) {
-          if (lane == 0 && abort_flag[1] == 0) abort_flag[1] = 4;
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t at = t_mine + static_cast<uint32_t>(acc * BN);
-        const uint64_t one_scale = pack2(rs * cs[0], rs * cs[0]);
-#pragma unroll
-        for (int c = 0; c < kCols; c += kChunk) {
-          uint32_t v[kChunk];
-          tmem_ld<kChunk>(at + c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < kChunk; e += 2) {
-            uint64_t s = one_scale;
-            if constexpr (VEC) {
-              // (a column's scale is held by one lane)
-              const float s0 = __shfl_sync(0xffffffffu, cs[c / 32], (c + e) & 31), s1 = __shfl_sync(0xffffffffu, cs[c / 32], (c + e + 1) & 31);
-              s = pack2(rs * s0, rs * s1);
-            }
-            sum[(c + e) / 2] = fma2(pack2(v[e], v[e + 1]), s, sum[(c + e) / 2]);
+        for (int e = 0; e < kChunk; e += 4) {
+          uint64_t s0 = row2, s1 = row2;
+          if constexpr (SCALES != kOfRows) {
+            const uint4 u = ld_shared_v4(scales + (c + e) * 4);
+            s0 = mul2(pack2(u.x, u.y), row2), s1 = mul2(pack2(u.z, u.w), row2);
           }
+          fma2(sum[(c + e) / 2], pack2(v[e], v[e + 1]), s0);
+          fma2(sum[(c + e) / 2 + 1], pack2(v[e + 2], v[e + 3]), s1);
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar(acc));
-        if (++acc == kAccs) acc = 0, acc_phase ^= 1u;
+      };
+      for (int kb = x.kb0; kb < x.kb1 && ok; ++kb) {
+        ok = ready();
+        if (!ok) break;
+        read_scales();
+        take_scales();
+        const uint32_t at = t_mine + static_cast<uint32_t>(acc * BN);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          uint32_t v[kChunk];
+          tmem_ld<kChunk>(at + c * kChunk, v);
+          tmem_ld_wait();
+          if (c == kChunks - 1) release();
+          add(v, c * kChunk);
+        }
       }
       if (!ok) break;
       if constexpr (SWAP) {
-        if (p.split > 1) {
+        if (Cfg::kSplits && p.split > 1) {
 #pragma unroll
           for (int j = 0; j < kCols / 2; ++j) {
             const float2 v = unpack2(sum[j]);
-            part[(half * kCols + 2 * j) * 128 + i] = v.x;
-            part[(half * kCols + 2 * j + 1) * 128 + i] = v.y;
+            part[(first_col + 2 * j) * 128 + i] = v.x;
+            part[(first_col + 2 * j + 1) * 128 + i] = v.y;
           }
         } else if (x.n0 + i < p.n) {
           const long long base = (p.terms ? x.group * p.stride_c : 0) + x.n0 + i;
 #pragma unroll
           for (int j = 0; j < kCols; ++j) {
             const float2 v = unpack2(sum[j / 2]);
-            const int row = x.row0 + half * kCols + j;
+            const int row = x.row0 + first_col + j;
             if (row < x.row_end) store_one(p, base + row * p.ldc, j & 1 ? v.y : v.x);
           }
         }
       } else {
-        const int row = x.row0 + i, col = x.n0 + half * kCols;
-        if (row < x.row_end) {
-          const long long base = (p.terms ? x.group * p.stride_c : 0) + row * p.ldc + col;
+        // The results are rounded into shared memory and leave by TMA while the warp goes on with the next tile (written by the
+        // warp itself, they held it up for 2 us per tile: no MMAs in that time, as both accumulators were full).
+        const int row = x.row0 + side * 128 + quarter * 32, col = x.n0 + first_col;
+        const int rows = min(x.row_end - row, 32);
+        const uint32_t at = out_stage + static_cast<uint32_t>(w) * 8192u;
+        const bool f32 = p.out_dtype == PMLB_F32;
+        // (a box that holds rows of the next group is stored row by row)
+        const bool by_tma = p.out_align >= 16 && (rows == 32 || x.row_end == p.m);
+        if (rows > 0) {
 #pragma unroll
-          for (int j = 0; j < kCols; j += 8) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float2 u = unpack2(sum[(j + e) / 2]);
-              v[e] = u.x, v[e + 1] = u.y;
+          for (int j = 0; j < kCols; j += 16) {
+            const int box = f32 ? j / 32 : j / 64;          // (two boxes of staging: f32 goes round it twice)
+            const uint32_t to = at + static_cast<uint32_t>(box & 1) * 4096u;
+            if (j % 64 == 0 && (j == 0 || f32)) {
+              if (lane == 0) bulk_wait_group_read<0>();
+              __syncwarp();
             }
-            if (col + j < p.n) store_eight(p, base + j, v, p.n - col - j);
+            uint32_t u[16];
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 t = unpack2(sum[(j + e) / 2]);
+              v[e] = t.x, v[e + 1] = t.y;
+            }
+            if (f32) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(v[e]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) st_shared_v4(to + box_piece(lane, j % 32 / 4 + e), make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) u[e] = p.out_dtype == PMLB_BF16 ? cvt_pack16<true, false>(v[2 * e], v[2 * e + 1]) : cvt_pack16<false, false>(v[2 * e], v[2 * e + 1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) st_shared_v4(to + box_piece(lane, j % 64 / 8 + e), make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]));
+            }
+            if (f32 ? j % 32 == 16 : j % 64 == 48) {
+              const int c0 = col + (f32 ? j - 16 : j - 48);   // the box's first column
+              if (c0 < p.n) {
+                // (a TMA store writes whole 16-byte units: a row that ends inside one would lose what lies behind it)
+                if (by_tma && (c0 + (f32 ? 32 : 64) <= p.n || p.n % (f32 ? 4 : 8) == 0)) {
+                  fence_proxy_async_smem();
+                  __syncwarp();
+                  if (lane == 0) {
+                    tma_store_3d(&map_c, to, c0, row, p.terms ? x.group : 0);
+                    bulk_commit_group();
+                  }
+                } else {
+                  __syncwarp();
+                  store_box(p, to, (p.terms ? x.group * p.stride_c : 0) + row * p.ldc + c0, rows, p.n - c0, lane);
+                }
+              }
+            }
           }
         }
       }
     }
+    if (lane == 0) bulk_wait_group_read<0>();   // (shared memory stays until the last box has left)
   }
 
   __syncwarp();
   tc_fence_before_sync();
-  if (p.split > 1) {
+  if (PAIR || p.split > 1) {
     cluster_sync_threads();
   } else {
     __syncthreads();
   }
   const bool failed = abort_flag[0] != 0;
-  if constexpr (SWAP) {
-    if (p.split > 1) {
+  if constexpr (Cfg::kSplits) {
+    if (p.split > 1 && first < total && !failed) {
       // The cluster's one tile: each CTA adds a run of its columns over all parts, in the order of the blocks.
-      if (first < total && !failed) {
-        const Tile x = tile_at(first);
-        const int begin = BN * 128 / p.split * rank, end = BN * 128 / p.split * (rank + 1);
-        const long long base = (p.terms ? x.group * p.stride_c : 0) + x.n0;
-        for (int e = begin + static_cast<int>(threadIdx.x); e < end; e += kThreads) {
-          const int j = e >> 7, i = e & 127;
-          const int row = x.row0 + j;
-          if (row >= x.row_end || x.n0 + i >= p.n) continue;
-          float v = 0.f;
-          for (int r = 0; r < p.split; ++r) v += ld_cluster_f32(mapa_rank(smem_u32(part + e), static_cast<uint32_t>(r)));
-          store_one(p, base + row * p.ldc + i, v);
-        }
+      const Tile x = tile_at(first);
+      const int begin = BN * 128 / p.split * rank, end = BN * 128 / p.split * (rank + 1);
+      const long long base = (p.terms ? x.group * p.stride_c : 0) + x.n0;
+      for (int e = begin + static_cast<int>(threadIdx.x); e < end; e += Cfg::kThreads) {
+        const int j = e >> 7, i = e & 127;
+        const int row = x.row0 + j;
+        if (row >= x.row_end || x.n0 + i >= p.n) continue;
+        float v = 0.f;
+        for (int r = 0; r < p.split; ++r) v += ld_cluster_f32(mapa_rank(smem_u32(part + e), static_cast<uint32_t>(r)));
+        store_one(p, base + row * p.ldc + i, v);
       }
-      cluster_sync_threads();   // no CTA leaves while another may still read its part
     }
   }
   if (failed) {
@@ -491,15 +687,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 2000000ull) __nanosleep(2000);
   }
-  __syncthreads();
+  __syncwarp();
+  if (PAIR || p.split > 1) {
+    cluster_sync_threads();   // no CTA leaves while another may still read its part, or before its MMAs have ended
+  } else {
+    __syncthreads();
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    if constexpr (PAIR) {
+      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    } else {
+      tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
   }
 }
 
-using KernelPtr = void (*)(const CUtensorMap, const CUtensorMap, const BlockGemmParams);
+using KernelPtr = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const BlockGemmParams);
 
 // The shared-memory limit is an attribute per device.
 template <class Cfg>
@@ -515,20 +720,21 @@ KernelPtr instance(int dev) {
 }
 
 template <class Cfg>
-cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const BlockGemmParams& p, int grid, int dev, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const CUtensorMap& mc, const BlockGemmParams& p, int grid, int dev, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(Cfg::kThreads);
   cfg.dynamicSmemBytes = Cfg::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0] = dependent_launch_attribute();
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.split;
+  const int share = Cfg::CTAS == 2 ? 2 : p.split;
+  attr[1].val.clusterDim.x = share;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, instance<Cfg>(dev), mp, mq, p);
+  cfg.numAttrs = share > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, instance<Cfg>(dev), mp, mq, mc, p);
 }
 
 uint32_t f8_format(int dtype) { return dtype == PMLB_F8E5M2 ? 1u : 0u; }
@@ -557,12 +763,11 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
 
   // Rows that a tile of tokens has to hold: those of the product, or of a group on average.
   const long long rows = by_rows ? (d.m + d.groups - 1) / d.groups : d.m;
-  const bool swap = rows <= 64;
-  int bn = 128;
-  if (swap) {
-    bn = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
-  }
-  const int tile_rows = swap ? bn : 128, tile_cols = swap ? 128 : bn;
+  const bool swap = rows <= 64, pair = !swap && rows > 128;
+  int bn = pair ? 256 : 128;
+  if (swap) bn = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  const int ctas = pair ? 2 : 1;
+  const int tile_rows = swap ? bn : 128 * ctas, tile_cols = swap ? 128 * ctas : bn;
   p.tiles_m = (d.m + tile_rows - 1) / tile_rows;
   p.tiles_n = (d.n + tile_cols - 1) / tile_cols;
   // (groups of rows: at most one tile more than whole ones for each group that has rows)
@@ -576,25 +781,35 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   if (swap) {
     while (p.split < 8 && tiles * p.split * 2 <= sms && p.num_kb >= p.split * 4) p.split *= 2;
   }
-  const int grid = p.split > 1 ? static_cast<int>(tiles) * p.split : static_cast<int>(std::min<long long>(tiles, sms));
+  const int grid = p.split > 1 ? static_cast<int>(tiles) * p.split : static_cast<int>(std::min<long long>(tiles, sms / ctas)) * ctas;
   // bits: [4,6) f32 accumulators, [7,10) and [10,13) formats of the two operands, [17,23) N >> 3, [24,29) M >> 4
   p.idesc = 1u << 4 | f8_format(swap ? d.b_dtype : d.a_dtype) << 7 | f8_format(swap ? d.a_dtype : d.b_dtype) << 10 |
-            static_cast<uint32_t>(bn >> 3) << 17 | 8u << 24;
+            static_cast<uint32_t>(bn >> 3) << 17 | static_cast<uint32_t>(8 * ctas) << 24;
 
-  CUtensorMap ma, mb;
-  if (!tc_encode_bytes(&ma, a, d.k, d.m, 1, d.lda, 16, tile_rows, err)) return PMLB_ERR_INVALID;
-  if (!tc_encode_bytes(&mb, b, d.k, d.n, by_rows ? d.groups : 1, d.ldb, by_rows ? d.stride_b : 16, tile_cols, err)) return PMLB_ERR_INVALID;
+  CUtensorMap ma, mb, mc;
+  std::memset(&mc, 0, sizeof(mc));
+  // (a CTA of a pair fetches 128 rows of one operand and its half of the other)
+  const int box_a = tile_rows / ctas, box_b = tile_cols / ctas;
+  if (!tc_encode_bytes(&ma, a, d.k, d.m, 1, d.lda, 16, box_a, err)) return PMLB_ERR_INVALID;
+  if (!tc_encode_bytes(&mb, b, d.k, d.n, by_rows ? d.groups : 1, d.ldb, by_rows ? d.stride_b : 16, box_b, err)) return PMLB_ERR_INVALID;
+  if (!swap && p.out_align >= 16 &&
+      !tc_encode_boxes(&mc, d.out_dtype, c, d.n, d.m, by_terms ? d.groups : 1, d.ldc, by_terms ? d.stride_c : 8, err)) {
+    return PMLB_ERR_INVALID;
+  }
   cudaError_t e = cudaSuccess;
+  const bool both = d.b_scale_rows == 1;   // rows and columns of a tile have scales of their own
   if (swap) {
-    switch (bn) {
-      case 16: e = launch<BlockCfg<16, true, true>>(mb, ma, p, grid, dev, stream); break;
-      case 32: e = launch<BlockCfg<32, true, true>>(mb, ma, p, grid, dev, stream); break;
-      default: e = launch<BlockCfg<64, true, true>>(mb, ma, p, grid, dev, stream); break;
+    if (bn == 16) {
+      e = both ? launch<BlockCfg<16, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream) : launch<BlockCfg<16, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
+    } else if (bn == 32) {
+      e = both ? launch<BlockCfg<32, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream) : launch<BlockCfg<32, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
+    } else {
+      e = both ? launch<BlockCfg<64, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream) : launch<BlockCfg<64, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
     }
-  } else if (d.b_scale_rows == 1) {
-    e = launch<BlockCfg<128, false, true>>(ma, mb, p, grid, dev, stream);
+  } else if (pair) {
+    e = both ? launch<BlockCfg<256, false, kOfBoth, 2>>(ma, mb, mc, p, grid, dev, stream) : launch<BlockCfg<256, false, kOfRows, 2>>(ma, mb, mc, p, grid, dev, stream);
   } else {
-    e = launch<BlockCfg<128, false, false>>(ma, mb, p, grid, dev, stream);
+    e = both ? launch<BlockCfg<128, false, kOfBoth>>(ma, mb, mc, p, grid, dev, stream) : launch<BlockCfg<128, false, kOfRows>>(ma, mb, mc, p, grid, dev, stream);
   }
   if (e != cudaSuccess) {
     *err = std::string("block_gemm launch: ") + cudaGetErrorString(e);

@@ -191,6 +191,13 @@ bool tc_encode_bytes(void* map, const void* base, long long d0, long long d1, lo
                   static_cast<uint32_t>(rows), 1, err);
 }
 
+bool tc_encode_boxes(void* map, int dtype, const void* base, long long d0, long long d1, long long d2, long long stride1, long long stride2,
+                     std::string* err) {
+  if (!tc_supported(err)) return false;
+  const int eb = out_bytes_of(dtype);
+  return encode3d(static_cast<CUtensorMap*>(map), out_map_dtype(dtype), eb, base, d0, d1, d2, stride1 * eb, stride2 * eb, 128 / eb, 32, 1, err);
+}
+
 int tc_launch(const TcLaunch& L, cudaStream_t stream, std::string* err) {
   load_driver_entry_points();
   if (!g_encode_tiled || !g_encode_im2col) {

@@ -111,5 +111,8 @@ bool tc_supported(std::string* why);
 // Tensor map of a [d2][d1][d0] tensor of bytes: boxes of 128 x `rows` bytes, 128-byte swizzle, zeros outside.  `map` is a CUtensorMap.
 bool tc_encode_bytes(void* map, const void* base, long long d0, long long d1, long long d2, long long stride1, long long stride2, int rows,
                      std::string* err);
+// The same of a [d2][d1][d0] tensor of F32, BF16 or F16, strides in elements, boxes of 32 rows of 128 bytes.
+bool tc_encode_boxes(void* map, int dtype, const void* base, long long d0, long long d1, long long d2, long long stride1, long long stride2,
+                     std::string* err);
 
 }  // namespace pmlb

@@ -1567,7 +1567,7 @@ std::string quant_problem(const pmlb_quant_desc& d) {
   if (d.ldx < d.cols || d.ldq < (turned ? d.rows : d.cols)) return "quant: a row stride smaller than a row";
   if (d.rows > (1 << 30) || d.cols > (1 << 30)) return "quant: sizes above 2^30";
   if (d.batch > 65535 || (d.form != PMLB_QUANT_ROWS && (d.rows + 127) / 128 > 65535)) return "quant: more rows or batch entries than one launch takes";
-  if (d.form == PMLB_QUANT_ROWS && ((d.cols + 511LL) / 512 * d.rows + 7) / 8 > 0x7fffffffLL) return "quant: more rows than one launch takes";
+  if (d.form == PMLB_QUANT_ROWS && d.cols > 65535 * 1024) return "quant: more columns than one launch takes";
   if (d.scale_row < 0 || d.scale_block < 0 || (d.batch > 1 && (d.stride_x < 0 || d.stride_q < 0 || d.stride_scale < 0))) return "quant: negative stride";
   if (d.source_rows < 0) return "quant: negative source_rows";
   if (d.source_rows > 0 && (d.form != PMLB_QUANT_ROWS || d.batch != 1)) return "quant: rows are taken by index in the form of rows, batch 1";

@@ -1719,15 +1719,13 @@ pmlb_status pmlb_route_invoke(pmlb_plan* plan, void* stream, const void* logits,
     return fail(PMLB_ERR_INVALID, "route: a pointer that is not aligned to its elements");
   }
   OnDevice on(plan->device);
+  cudaError_t e = cudaSuccess;
   if (d.tokens > 0) {
-    const cudaError_t e = pmlb::launch_route(d, logits, bias, weights, ids, static_cast<cudaStream_t>(stream));
-    if (e != cudaSuccess) return cuda_fail(e, "route launch");
+    e = pmlb::launch_route(d, logits, bias, weights, ids, offsets, source, position, static_cast<cudaStream_t>(stream));
+  } else if (d.rows > 0) {
+    e = pmlb::launch_route_order(d, ids, offsets, source, position, static_cast<cudaStream_t>(stream));
   }
-  if (d.rows > 0) {
-    const cudaError_t e = pmlb::launch_route_order(d, ids, offsets, source, position, static_cast<cudaStream_t>(stream));
-    if (e != cudaSuccess) return cuda_fail(e, "route order launch");
-  }
-  return PMLB_OK;
+  return e == cudaSuccess ? PMLB_OK : cuda_fail(e, "route launch");
 }
 
 pmlb_status pmlb_route_grad(pmlb_plan* plan, void* stream, const void* logits, const int32_t* ids, const float* dweights,

@@ -3,8 +3,9 @@
 //   out[t] = sum_j w[t, j] * y[position[t, j]]
 //   dy[position[t, j]] = w[t, j] * dout[t],   dw[t, j] = <dout[t], y[position[t, j]]>
 //
-// Memory-bound: each row of y is read once, each row of out (dout) written (read) once.  A block takes one token; the rows of
-// its choices are loaded together, 16 bytes per lane.
+// Bound by memory: each row of y is read once, each row of out (dout) written (read) once.  A block takes one token, a thread 16
+// bytes of a row at a time; what keeps the memory busy is that a thread's loads of up to eight rows are on their way
+// together, so they are not made conditional: a pair without a row reads row 0 and leaves it out.
 #include "combine.h"
 
 #include <cuda_bf16.h>
@@ -17,8 +18,8 @@
 namespace pmlb {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kAtOnce = 4;   // rows in flight per thread
+constexpr int kThreads = 256, kGradThreads = 128;
+constexpr int kRowsPerWarp = 4;
 
 struct CombineParams {
   const void *y, *dout;
@@ -26,7 +27,7 @@ struct CombineParams {
   const int32_t *position, *source;
   void *out, *dy;
   float* dweights;
-  int tokens, top_k, width, rows;
+  int tokens, top_k, width, rows, row_blocks;
   long long ldy, ldo;
 };
 
@@ -54,58 +55,134 @@ struct __align__(sizeof(T) * N) Pack {
   T e[N];
 };
 
+template <class P>
+__device__ __forceinline__ P load_once(const void* at) {   // (read once: no place in L1)
+  if constexpr (sizeof(P) == 16) {
+    uint4 u;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(at));
+    return *reinterpret_cast<const P*>(&u);
+  } else {
+    return *static_cast<const P*>(at);
+  }
+}
+
+// Adds U of the token's rows, from choice j on, to the sums of columns c, c + 1, ..
+template <class T, int N, int U>
+__device__ __forceinline__ void add_rows(const CombineParams& p, const int32_t* position, const float* weights, int j, int c, float (&sum)[N]) {
+  using P = Pack<T, N>;
+  P row[U];
+  float w[U];
+  bool there[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int r = __ldg(position + j + u);
+    there[u] = static_cast<unsigned>(r) < static_cast<unsigned>(p.rows);
+    row[u] = load_once<P>(static_cast<const T*>(p.y) + (there[u] ? r * p.ldy : 0) + c);
+    w[u] = weights != nullptr ? __ldg(weights + j + u) : 1.f;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float v = fmaf(w[u], Elem<T>::get(row[u].e[e]), sum[e]);
+      sum[e] = there[u] ? v : sum[e];
+    }
+  }
+}
+
 template <class T, int N>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const CombineParams p) {
-  using P = Pack<T, N>;
   dependent_entry();
   const long long t = blockIdx.x;
   const int32_t* position = p.position + t * p.top_k;
-  const T* y = static_cast<const T*>(p.y);
+  const float* weights = p.weights != nullptr ? p.weights + t * p.top_k : nullptr;
   T* out = static_cast<T*>(p.out) + t * p.ldo;
   for (int c = threadIdx.x * N; c < p.width; c += kThreads * N) {
     float sum[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) sum[e] = 0.f;
-    for (int j0 = 0; j0 < p.top_k; j0 += kAtOnce) {
-      P row[kAtOnce];
-      float w[kAtOnce];
-      bool there[kAtOnce];
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        const int r = j0 + u < p.top_k ? __ldg(position + j0 + u) : -1;
-        there[u] = static_cast<unsigned>(r) < static_cast<unsigned>(p.rows);
-        if (there[u]) {
-          row[u] = *reinterpret_cast<const P*>(y + r * p.ldy + c);
-          w[u] = p.weights != nullptr ? __ldg(p.weights + t * p.top_k + j0 + u) : 1.f;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) {
-        if (!there[u]) continue;
-#pragma unroll
-        for (int e = 0; e < N; ++e) sum[e] = fmaf(w[u], Elem<T>::get(row[u].e[e]), sum[e]);
-      }
-    }
-    P o;
+    int j = p.rows > 0 ? 0 : p.top_k;   // (without rows there is nothing to read, not even row 0)
+    for (; j + 8 <= p.top_k; j += 8) add_rows<T, N, 8>(p, position, weights, j, c, sum);
+    if (j + 4 <= p.top_k) add_rows<T, N, 4>(p, position, weights, j, c, sum), j += 4;
+    if (j + 2 <= p.top_k) add_rows<T, N, 2>(p, position, weights, j, c, sum), j += 2;
+    if (j < p.top_k) add_rows<T, N, 1>(p, position, weights, j, c, sum);
+    Pack<T, N> o;
 #pragma unroll
     for (int e = 0; e < N; ++e) o.e[e] = Elem<T>::put(sum[e]);
-    *reinterpret_cast<P*>(out + c) = o;
+    *reinterpret_cast<Pack<T, N>*>(out + c) = o;
   }
 }
 
-// Blocks [0, tokens): a token's rows.  The blocks behind them write zeros to rows that no pair has.
-template <class T, int N>
-__global__ void __launch_bounds__(kThreads) combine_grad_kernel(const CombineParams p) {
+// The gradients of U of token t's choices, from choice j on.  `part`: [warps][8] in shared memory.
+template <class T, int N, int U>
+__device__ __forceinline__ void grad_rows(const CombineParams& p, long long t, int j, float (*part)[8]) {
   using P = Pack<T, N>;
-  __shared__ float part[kThreads / 32];
-  dependent_entry();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x >= static_cast<unsigned>(p.tokens)) {
-    const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
-    const int r0 = (blockIdx.x - p.tokens) * kThreads + warp * 32;
-    int pair = 0;
-    if (r0 + lane < p.rows) pair = __ldg(p.source + r0 + lane);
-    unsigned empty = __ballot_sync(0xffffffffu, r0 + lane < p.rows && (pair < 0 || pair >= pairs));
+  const T* dout = static_cast<const T*>(p.dout) + t * p.ldo;
+  const bool dots = p.dweights != nullptr && p.rows > 0;
+  int at[U];
+  float w[U], dot[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    at[u] = __ldg(p.position + t * p.top_k + j + u);
+    w[u] = p.weights != nullptr ? __ldg(p.weights + t * p.top_k + j + u) : 1.f;
+    dot[u] = 0.f;
+  }
+  auto there = [&](int u) { return static_cast<unsigned>(at[u]) < static_cast<unsigned>(p.rows); };
+  for (int c = threadIdx.x * N; c < p.width; c += kGradThreads * N) {
+    P row[U];
+    const P g = load_once<P>(dout + c);
+    if (dots) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) row[u] = load_once<P>(static_cast<const T*>(p.y) + (there(u) ? at[u] * p.ldy : 0) + c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (dots) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) dot[u] = fmaf(Elem<T>::get(g.e[e]), Elem<T>::get(row[u].e[e]), dot[u]);
+      }
+      if (p.dy != nullptr && there(u)) {
+        P o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.e[e] = Elem<T>::put(w[u] * Elem<T>::get(g.e[e]));
+        *reinterpret_cast<P*>(static_cast<T*>(p.dy) + at[u] * p.ldy + c) = o;
+      }
+    }
+  }
+  if (p.dweights == nullptr) return;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], d);
+  }
+  __syncthreads();   // (the sums of the choices before have been read)
+  if (lane == 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) part[warp][u] = there(u) ? dot[u] : 0.f;
+  }
+  __syncthreads();
+  if (threadIdx.x < U) {
+    float all = 0.f;
+#pragma unroll
+    for (int i = 0; i < kGradThreads / 32; ++i) all += part[i][threadIdx.x];
+    p.dweights[t * p.top_k + j + threadIdx.x] = all;
+  }
+}
+
+// Blocks [0, row_blocks): zeros for rows that no pair has (first, and few rows per warp: the rows behind the last segment lie
+// together, and a warp with many of them would end long after the others).  The others: a token each.
+template <class T, int N>
+__global__ void __launch_bounds__(kGradThreads) combine_grad_kernel(const CombineParams p) {
+  using P = Pack<T, N>;
+  __shared__ float part[kGradThreads / 32][8];
+  dependent_entry();
+  if (blockIdx.x < static_cast<unsigned>(p.row_blocks)) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r0 = (blockIdx.x * (kGradThreads / 32) + warp) * kRowsPerWarp;
+    const bool mine = lane < kRowsPerWarp && r0 + lane < p.rows;
+    const int pair = mine ? __ldg(p.source + r0 + lane) : 0;
+    unsigned empty = __ballot_sync(0xffffffffu, mine && static_cast<unsigned>(pair) >= static_cast<unsigned>(p.tokens) * p.top_k);
     P zero;
 #pragma unroll
     for (int e = 0; e < N; ++e) zero.e[e] = Elem<T>::put(0.f);
@@ -116,54 +193,27 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const CombinePar
     }
     return;
   }
-  const long long t = blockIdx.x;
-  const T* dout = static_cast<const T*>(p.dout) + t * p.ldo;
-  for (int j = 0; j < p.top_k; ++j) {
-    const int r = __ldg(p.position + t * p.top_k + j);
-    const bool there = static_cast<unsigned>(r) < static_cast<unsigned>(p.rows);
-    const float w = p.weights != nullptr ? __ldg(p.weights + t * p.top_k + j) : 1.f;
-    float dot = 0.f;
-    if (there) {
-      for (int c = threadIdx.x * N; c < p.width; c += kThreads * N) {
-        const P g = *reinterpret_cast<const P*>(dout + c);
-        if (p.dweights != nullptr) {
-          const P v = *reinterpret_cast<const P*>(static_cast<const T*>(p.y) + r * p.ldy + c);
-#pragma unroll
-          for (int e = 0; e < N; ++e) dot = fmaf(Elem<T>::get(g.e[e]), Elem<T>::get(v.e[e]), dot);
-        }
-        if (p.dy != nullptr) {
-          P o;
-#pragma unroll
-          for (int e = 0; e < N; ++e) o.e[e] = Elem<T>::put(w * Elem<T>::get(g.e[e]));
-          *reinterpret_cast<P*>(static_cast<T*>(p.dy) + r * p.ldy + c) = o;
-        }
-      }
-    }
-    if (p.dweights != nullptr) {
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-      __syncthreads();
-      if (lane == 0) part[warp] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        float all = 0.f;
-        for (int i = 0; i < kThreads / 32; ++i) all += part[i];
-        p.dweights[t * p.top_k + j] = all;
-      }
-    }
-  }
+  const long long t = blockIdx.x - p.row_blocks;
+  int j = 0;
+  for (; j + 8 <= p.top_k; j += 8) grad_rows<T, N, 8>(p, t, j, part);
+  if (j + 4 <= p.top_k) grad_rows<T, N, 4>(p, t, j, part), j += 4;
+  if (j + 2 <= p.top_k) grad_rows<T, N, 2>(p, t, j, part), j += 2;
+  if (j < p.top_k) grad_rows<T, N, 1>(p, t, j, part);
 }
 
 template <class T>
-cudaError_t launch_typed(const CombineParams& p, bool grad, cudaStream_t stream) {
+cudaError_t launch_typed(CombineParams p, bool grad, cudaStream_t stream) {
   constexpr int kWide = 16 / sizeof(T);
   auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   const bool wide = p.width % kWide == 0 && p.ldy % kWide == 0 && p.ldo % kWide == 0 && aligned(p.y) && aligned(p.dout) && aligned(p.out) &&
                     aligned(p.dy);
-  unsigned grid = static_cast<unsigned>(p.tokens);
-  if (!grad) return launch_dependent(wide ? combine_kernel<T, kWide> : combine_kernel<T, 1>, dim3(grid), kThreads, stream, p);
-  if (p.dy != nullptr) grid += (p.rows + kThreads - 1) / kThreads;
-  return launch_dependent(wide ? combine_grad_kernel<T, kWide> : combine_grad_kernel<T, 1>, dim3(grid), kThreads, stream, p);
+  if (!grad) {
+    return launch_dependent(wide ? combine_kernel<T, kWide> : combine_kernel<T, 1>, dim3(static_cast<unsigned>(p.tokens)), kThreads, stream, p);
+  }
+  constexpr int kRows = kGradThreads / 32 * kRowsPerWarp;
+  p.row_blocks = p.dy != nullptr ? (p.rows + kRows - 1) / kRows : 0;
+  const dim3 grid(static_cast<unsigned>(p.row_blocks + p.tokens));
+  return launch_dependent(wide ? combine_grad_kernel<T, kWide> : combine_grad_kernel<T, 1>, grid, kGradThreads, stream, p);
 }
 
 cudaError_t launch_of(int dtype, const CombineParams& p, bool grad, cudaStream_t stream) {

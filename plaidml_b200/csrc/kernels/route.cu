@@ -91,10 +91,14 @@ __device__ __forceinline__ float warp_max(float v) {   // (NaN does not count)
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
   return y;
 }
+// By integers of the same order, the upper half first: two reductions in hardware where shuffles would be ten.
 __device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = larger(v, __shfl_xor_sync(kAll, v, d));
-  return v;
+  const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(v));
+  const unsigned long long key = v != v ? 0ull : ((bits >> 63) != 0 ? ~bits : bits | (1ull << 63));
+  const unsigned hi = static_cast<unsigned>(key >> 32), lo = static_cast<unsigned>(key);
+  const unsigned top = __reduce_max_sync(kAll, hi), low = __reduce_max_sync(kAll, hi == top ? lo : 0u);
+  const unsigned long long most = static_cast<unsigned long long>(top) << 32 | low;
+  return __longlong_as_double(static_cast<long long>((most >> 63) != 0 ? most & ~(1ull << 63) : ~most));
 }
 
 // Scores of the row; -infinity scores 0 whatever the others are.
@@ -252,17 +256,14 @@ __device__ __forceinline__ bool choose(const RouteParams& p, const float (&z)[N]
     for (int i = 1; i < N; ++i) v = larger(v, r[i]);
     return v;
   };
-  F v = best(), last = 0;   // this lane's largest that is left, NaN for none
+  F v = best(), value_of_mine = 0;   // this lane's largest that is left, NaN for none; the value of the lane-th choice
   *mine = -1;
-  const int picks = p.top_k + (kExact || plain || p.top_k == p.experts ? 0 : 1);   // (the first one left out tells how near it was)
+  // (the first one left out tells how near it was)
+  const int picks = p.top_k + (kExact || plain || p.top_k == p.experts ? 0 : 1);
+  F most = 0;
   for (int j = 0; j < picks; ++j) {
-    const F most = warp_max(v);
+    most = warp_max(v);
     const int from = __ffs(__ballot_sync(kAll, v == most)) - 1;
-    if (!kExact && !plain && j > 0) {
-      const F size = larger(last < 0 ? -last : last, most < 0 ? -most : most);
-      if (last - most <= base + 2 * u * size) close = true;
-    }
-    last = most;
     int at = 0;
     if (lane == from) {
       // the first of its registers that holds it is taken
@@ -276,7 +277,14 @@ __device__ __forceinline__ bool choose(const RouteParams& p, const float (&z)[N]
       v = best();
     }
     const int e = __shfl_sync(kAll, at, from);
-    if (lane == j && j < p.top_k) *mine = e;
+    if (lane == j) *mine = e, value_of_mine = most;
+  }
+  if (!kExact && !plain) {
+    // each choice with the one after it
+    F next = __shfl_down_sync(kAll, value_of_mine, 1);
+    if (lane == p.top_k - 1) next = most;   // (lane 31 has none after it)
+    const F size = larger(value_of_mine < 0 ? -value_of_mine : value_of_mine, next < 0 ? -next : next);
+    if (__any_sync(kAll, lane + 1 < picks && value_of_mine - next <= base + 2 * u * size)) close = true;
   }
   return close;
 }
@@ -476,25 +484,41 @@ __device__ __forceinline__ void order_pairs(const OrderParams& p, uint32_t* coun
   int kept[kKeep];   // ids, then rank << 10 | id, -1 for pairs without an expert
 #pragma unroll
   for (int k = 0; k < kKeep; ++k) kept[k] = begin + k * 32 + lane < end ? p.ids[begin + k * 32 + lane] : -1;
-  for (int e = threadIdx.x; e < kOrderWarps * p.experts; e += kOrderThreads) counts[e] = 0;
+  for (int e = threadIdx.x; e < kOrderWarps * p.experts; e += kOrderThreads) {
+    counts[e] = 0;
+    if (kOrderWarps * p.experts * 4 <= kStaged * 6) staged[e] = 0;
+  }
   __syncthreads();
   uint32_t* my = counts + warp * p.experts;
-  // (lanes of the same expert by a vote per bit of the id: 16.2 us for 131072 pairs of 256 experts, 18.8 with match.any.  Ranks
-  // stay below the 2^24 pairs divided by the 256 runs that more than 1024 pairs are cut into: 16 bits)
+  // Lanes of the same expert: each sets its bit in the expert's word of the warp (in the place of the staged pairs, which come
+  // later), or, for more experts than there is room for, a vote per bit of the id.  (131072 pairs of 256 experts: 18.8 us with
+  // match.any, 14.5 with votes, 11.6 with the words.)  Ranks stay below the 2^24 pairs divided by the 256 runs that more
+  // than 1024 pairs are cut into: 16 bits.
+  const bool by_words = kOrderWarps * p.experts * 4 <= kStaged * 6;
+  uint32_t* words = staged + warp * p.experts;
   const int id_bits = 32 - __clz(p.experts);
   auto ranked = [&](int id) {
     const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(p.experts);
-    const int key = there ? id : p.experts;
     unsigned same = kAll;
-    for (int b = 0; b < id_bits; ++b) {
-      const bool bit = (key >> b) & 1;
-      const unsigned m = __ballot_sync(kAll, bit);
-      same &= bit ? m : ~m;
+    if (by_words) {
+      if (there) atomicOr(words + id, 1u << lane);
+      __syncwarp();
+      if (there) same = words[id];
+    } else {
+      const int key = there ? id : p.experts;
+      for (int b = 0; b < id_bits; ++b) {
+        const bool bit = (key >> b) & 1;
+        const unsigned m = __ballot_sync(kAll, bit);
+        same &= bit ? m : ~m;
+      }
     }
     uint32_t r = 0;
     if (there) r = my[id] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
-    if (there && (same >> lane) == 1u) my[id] = r + 1;   // the last lane of its expert
+    if (there && (same >> lane) == 1u) {   // the last lane of its expert
+      my[id] = r + 1;
+      if (by_words) words[id] = 0;
+    }
     __syncwarp();
     return there ? static_cast<int>(r << 10 | static_cast<uint32_t>(id)) : -1;
   };

@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 
@@ -46,11 +47,11 @@ struct BlockCfg {
   static constexpr int kStageBytes = kTileP + kTileQ;
   static constexpr int kAccs = BN == 256 ? 2 : 4;
   static constexpr int kTmemCols = kAccs * BN;
-  static constexpr bool kSplits = kSwap && CTAS == 1;                               // K may be shared by a cluster
-  static constexpr int kPartBytes = kSplits ? BN * 128 * 4 : 0;                     // this CTA's sums, where it is
+  static constexpr bool kSplits = CTAS == 1;                                        // K may be shared by a cluster
+  static constexpr int kPartBytes = kSwap ? BN * 128 * 4 : 0;                       // this CTA's sums, where it is (else in the place of the boxes)
   // Scales of a block: one for each row of the accumulator, then one for each column (or for each 128 of them); kAhead blocks are
   // on their way (see the warp that fetches them for what bounds it).
-  static constexpr int kSlots = kScales == kOfBoth && BN == 256 ? 8 : 16, kAhead = kSlots - 2 * kAccs - 1;
+  static constexpr int kSlots = 16, kAhead = kSlots - 2 * kAccs - 1;
   static constexpr int kSlotFloats = 128 + (kScales == kOfBoth ? BN : 4);
   static constexpr int kScaleBytes = kSlots * kSlotFloats * 4;
   static constexpr int kStageOutBytes = kSwap ? 0 : kSumWarps * 8192;    // results on their way out: two boxes of 32 rows of 128 bytes per warp
@@ -58,6 +59,7 @@ struct BlockCfg {
   static constexpr int kStages = std::min(10, (232448 - 1024 - kPartBytes - kScaleBytes - kStageOutBytes - kTailBytes) / kStageBytes);
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kPartBytes + kScaleBytes + kStageOutBytes + kTailBytes;
   static_assert(kStages >= 3 && kSmem <= 232448, "shared memory");
+  static_assert(kSwap || !kSplits || kStageOutBytes >= BN * 128 * 4, "room for a part");
 };
 
 struct BlockGemmParams {
@@ -152,6 +154,12 @@ __device__ __forceinline__ void copy_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
 // All threads of the cluster, from code where the warp's lanes may have parted.
 __device__ __forceinline__ void cluster_sync_threads() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
@@ -166,6 +174,30 @@ __device__ __forceinline__ void store_one(const BlockGemmParams& p, long long at
     static_cast<__half*>(p.out)[at] = __float2half_rn(v);
   }
 }
+
+// Four consecutive columns of a row from element `at` on, `n` of which exist.
+__device__ __forceinline__ void store_four(const BlockGemmParams& p, long long at, const float4& v, int n) {
+  if (n >= 4 && p.out_align >= 16) {
+    if (p.out_dtype == PMLB_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+    } else {
+      const bool bf16 = p.out_dtype == PMLB_BF16;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+          make_uint2(bf16 ? cvt_pack16<true, false>(v.x, v.y) : cvt_pack16<false, false>(v.x, v.y),
+                     bf16 ? cvt_pack16<true, false>(v.z, v.w) : cvt_pack16<false, false>(v.z, v.w));
+    }
+  } else {
+    const float one[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e < n) store_one(p, at + e, one[e]);
+    }
+  }
+}
+
+// Part of a tile in shared memory: rows of BN floats, 16-byte pieces permuted by the row (a lane writes a row).
+template <int BN>
+__device__ __forceinline__ uint32_t part_piece(uint32_t row, uint32_t piece) { return row * (BN * 4u) + ((piece ^ (row & 7u)) << 4); }
 
 // Results leave through shared memory in boxes of 32 rows of 128 bytes (64 columns of 16 bits, or 32 of 32 bits), in the layout
 // of a TMA store with 128-byte swizzle: 16-byte pieces permuted by the row, which spreads a lane's row over the banks.
@@ -222,9 +254,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   uint8_t* tail = after_ring + Cfg::kPartBytes + Cfg::kScaleBytes;
   const uint32_t bar0 = smem_u32(tail);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (10 + s); };
-  auto tfull_bar = [&](int a) { return bar0 + 8u * (20 + a); };
-  auto tempty_bar = [&](int a) { return bar0 + 8u * (24 + a); };
+  auto done_bar = [&](int s) { return bar0 + 8u * (10 + s); };     // the stage's products (and their scales) are there, its operands free
+  auto tempty_bar = [&](int a) { return bar0 + 8u * (20 + a); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 264);   // flag, code, wait limit
   int* begins = reinterpret_cast<int*>(tail + 512);         // groups of rows: first row (and, behind the last one, the end),
@@ -236,10 +267,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   if (threadIdx.x == 64) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(done_bar(s), 2);   // (the products, and their scales)
     }
     for (int a = 0; a < kAccs; ++a) {
-      mbar_init(tfull_bar(a), 2);   // (the products, and their scales)
       mbar_init(tempty_bar(a), Cfg::kSumWarps * CTAS);   // (pairs: both CTAs' warps, at the first CTA)
     }
     abort_flag[0] = 0;
@@ -363,7 +393,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         const int py = (SWAP ? x.n0 : x.row0) + side * 128, qy = (SWAP ? x.row0 : x.n0) + side * (BN / CTAS);
         const int z = p.terms ? 0 : x.group;
         for (int kb = x.kb0; kb < x.kb1; ++kb) {
-          if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag)) {
+          if (!mbar_wait_warp(done_bar(stage), phase ^ 1u, abort_flag)) {
             if (leader && abort_flag[1] == 0) abort_flag[1] = 1;
             ok = false;
             break;
@@ -395,28 +425,29 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       for (int t = first; t < total && ok; t += units) {
         const Tile x = tile_at(t);
         for (int kb = x.kb0; kb < x.kb1; ++kb) {
-          // (the accumulator last: it is what the loop waits for)
-          if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) {
-            if (leader && abort_flag[1] == 0) abort_flag[1] = 3;
-            ok = false;
-            break;
-          }
+          // (both barriers are asked before either answer is waited for, and one commit serves the loaders and the adding warps)
           const uint32_t s = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
           const uint32_t lo_p = desc_lo | ((s & 0x3FFFFu) >> 4), lo_q = desc_lo | (((s + Cfg::kTileP) & 0x3FFFFu) >> 4);
-          if (!mbar_wait_warp(tempty_bar(acc), acc_phase ^ 1u, abort_flag)) {
-            if (leader && abort_flag[1] == 0) abort_flag[1] = 2;
-            ok = false;
-            break;
+          const bool both = mbar_test_wait(full_bar(stage), phase) & mbar_test_wait(tempty_bar(acc), acc_phase ^ 1u);
+          if (!__all_sync(0xffffffffu, both)) {
+            if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) {
+              if (leader && abort_flag[1] == 0) abort_flag[1] = 3;
+              ok = false;
+              break;
+            }
+            if (!mbar_wait_warp(tempty_bar(acc), acc_phase ^ 1u, abort_flag)) {
+              if (leader && abort_flag[1] == 0) abort_flag[1] = 2;
+              ok = false;
+              break;
+            }
           }
           tc_fence_after_sync();
           if (leader) {
             tc_mma_x4<kMmaF8, CTAS>(tmem_base + static_cast<uint32_t>(acc * BN), lo_p, lo_q, desc_hi, desc_hi, p.idesc, 0u, 2u, 2u);
             if constexpr (PAIR) {
-              tc_commit_pair(tfull_bar(acc), 3);
-              tc_commit_pair(empty_bar(stage), 3);
+              tc_commit_pair(done_bar(stage), 3);
             } else {
-              tc_commit(tfull_bar(acc));
-              tc_commit(empty_bar(stage));
+              tc_commit(done_bar(stage));
             }
           }
           __syncwarp();
@@ -476,22 +507,27 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       };
       point_at(first);
       for (int e = 0; e < Cfg::kAhead; ++e) request();
-      int acc = 0;
-      uint32_t acc_phase = 0;
+      int stage = 0, old_stage = 0, step = 0;   // of this block, and of the block kAccs before it
+      uint32_t old_phase = 0;
       bool ok = true;
       for (int t = first; t < total && ok; t += units) {
         const Tile x = tile_at(t);
         for (int kb = x.kb0; kb < x.kb1; ++kb) {
-          if (!mbar_wait_warp(tfull_bar(acc), acc_phase ^ 1u, abort_flag)) {
-            if (lane == 0 && abort_flag[1] == 0) abort_flag[1] = 5;
-            ok = false;
-            break;
+          if (step < kAccs) {
+            ++step;
+          } else {
+            if (!mbar_wait_warp(done_bar(old_stage), old_phase, abort_flag)) {
+              if (lane == 0 && abort_flag[1] == 0) abort_flag[1] = 5;
+              ok = false;
+              break;
+            }
+            if (++old_stage == kStages) old_stage = 0, old_phase ^= 1u;
           }
           request();
           copy_async_wait<Cfg::kAhead>();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tfull_bar(acc));
-          if (++acc == kAccs) acc = 0, acc_phase ^= 1u;
+          if (lane == 0) mbar_arrive(done_bar(stage));
+          if (++stage == kStages) stage = 0;
         }
       }
       copy_async_wait<0>();
@@ -507,16 +543,17 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     // of 32 73; a weight gradient's two scales per element: 100, 107, 120).
     constexpr int kChunk = kCols < 16 ? kCols : (SCALES == kOfRows && kCols >= 64 ? 64 : 16), kChunks = kCols / kChunk;
     const uint32_t t_mine = tmem_base + static_cast<uint32_t>(first_col) + (static_cast<uint32_t>(quarter * 32) << 16);
-    int acc = 0, slot = 0;
-    uint32_t acc_phase = 0;
+    int acc = 0, slot = 0, stage = 0;
+    uint32_t phase = 0;
     bool ok = true;
     const uint32_t tempty_at_first = PAIR ? mapa_rank(tempty_bar(0), 0) : 0u;
     // Waits for the accumulator's block and its scales; false: gave up.
     auto ready = [&]() {
-      if (!mbar_wait_warp(tfull_bar(acc), acc_phase, abort_flag)) {
+      if (!mbar_wait_warp(done_bar(stage), phase, abort_flag)) {
         if (lane == 0 && abort_flag[1] == 0) abort_flag[1] = 4;
         return false;
       }
+      if (++stage == kStages) stage = 0, phase ^= 1u;
       tc_fence_after_sync();
       return true;
     };
@@ -531,7 +568,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
           mbar_arrive(tempty_bar(acc));
         }
       }
-      if (++acc == kAccs) acc = 0, acc_phase ^= 1u;
+      if (++acc == kAccs) acc = 0;
     };
     for (int t = first; t < total && ok; t += units) {
       const Tile x = tile_at(t);
@@ -539,17 +576,14 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       uint64_t sum[kCols / 2];
 #pragma unroll
       for (int j = 0; j < kCols / 2; ++j) sum[j] = 0;
-      float next_row = 0.f;    // the row's scale (kOfRows: times that of the columns) of the block that is ready
-      uint64_t row2 = 0;       // ... and of the one that is being added
+      uint64_t row2 = 0;       // the row's scale (kOfRows: times that of the columns)
       uint32_t scales = 0;     // the columns' ones
-      auto read_scales = [&]() {
-        const uint32_t at = scale_ring + static_cast<uint32_t>(slot * Cfg::kSlotFloats * 4);
-        next_row = ld_shared_f32(at + (quarter * 32 + lane) * 4);
-        if constexpr (SCALES == kOfRows) next_row *= ld_shared_f32(at + 512u + (first_col / 128) * 4);
-      };
       auto take_scales = [&]() {
-        row2 = pack2(next_row, next_row);
-        scales = scale_ring + static_cast<uint32_t>(slot * Cfg::kSlotFloats * 4) + 512u + first_col * 4;
+        const uint32_t at = scale_ring + static_cast<uint32_t>(slot * Cfg::kSlotFloats * 4);
+        float rs = ld_shared_f32(at + (quarter * 32 + lane) * 4);
+        if constexpr (SCALES == kOfRows) rs *= ld_shared_f32(at + 512u + (first_col / 128) * 4);
+        row2 = pack2(rs, rs);
+        scales = at + 512u + first_col * 4;
         if (++slot == Cfg::kSlots) slot = 0;
       };
       auto add = [&](uint32_t (&v)[kChunk], int c) {
@@ -567,13 +601,12 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       for (int kb = x.kb0; kb < x.kb1 && ok; ++kb) {
         ok = ready();
         if (!ok) break;
-        read_scales();
-        take_scales();
         const uint32_t at = t_mine + static_cast<uint32_t>(acc * BN);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           uint32_t v[kChunk];
           tmem_ld<kChunk>(at + c * kChunk, v);
+          if (c == 0) take_scales();
           tmem_ld_wait();
           if (c == kChunks - 1) release();
           add(v, c * kChunk);
@@ -598,6 +631,15 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
           }
         }
       } else {
+        if (Cfg::kSplits && p.split > 1) {
+#pragma unroll
+          for (int j = 0; j < kCols; j += 4) {
+            const float2 a = unpack2(sum[j / 2]), b = unpack2(sum[j / 2 + 1]);
+            st_shared_v4(out_stage + part_piece<BN>(i, (first_col + j) / 4),
+                         make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)));
+          }
+          continue;
+        }
         // The results are rounded into shared memory and leave by TMA while the warp goes on with the next tile (written by the
         // warp itself, they held it up for 2 us per tile: no MMAs in that time, as both accumulators were full).
         const int row = x.row0 + side * 128 + quarter * 32, col = x.n0 + first_col;
@@ -667,17 +709,38 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   const bool failed = abort_flag[0] != 0;
   if constexpr (Cfg::kSplits) {
     if (p.split > 1 && first < total && !failed) {
-      // The cluster's one tile: each CTA adds a run of its columns over all parts, in the order of the blocks.
+      // The cluster's one tile: each CTA adds a run of its rows (SWAP: columns of the accumulator, which are rows of C) over all
+      // parts, in the order of the blocks.
       const Tile x = tile_at(first);
-      const int begin = BN * 128 / p.split * rank, end = BN * 128 / p.split * (rank + 1);
-      const long long base = (p.terms ? x.group * p.stride_c : 0) + x.n0;
-      for (int e = begin + static_cast<int>(threadIdx.x); e < end; e += Cfg::kThreads) {
-        const int j = e >> 7, i = e & 127;
-        const int row = x.row0 + j;
-        if (row >= x.row_end || x.n0 + i >= p.n) continue;
-        float v = 0.f;
-        for (int r = 0; r < p.split; ++r) v += ld_cluster_f32(mapa_rank(smem_u32(part + e), static_cast<uint32_t>(r)));
-        store_one(p, base + row * p.ldc + i, v);
+      if constexpr (SWAP) {
+        const int begin = BN * 128 / p.split * rank, end = BN * 128 / p.split * (rank + 1);
+        const long long base = (p.terms ? x.group * p.stride_c : 0) + x.n0;
+        for (int e = begin + static_cast<int>(threadIdx.x); e < end; e += Cfg::kThreads) {
+          const int j = e >> 7, i = e & 127;
+          const int row = x.row0 + j;
+          if (row >= x.row_end || x.n0 + i >= p.n) continue;
+          float v[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) v[r] = r < p.split ? ld_cluster_f32(mapa_rank(smem_u32(part + e), static_cast<uint32_t>(r))) : 0.f;
+#pragma unroll
+          for (int r = 1; r < 8; ++r) v[0] += v[r];
+          store_one(p, base + row * p.ldc + i, v[0]);
+        }
+      } else {
+        constexpr int kPieces = BN / 4;
+        const int begin = 128 / p.split * rank * kPieces, end = 128 / p.split * (rank + 1) * kPieces;
+        const long long base = p.terms ? x.group * p.stride_c : 0;
+        for (int e = begin + static_cast<int>(threadIdx.x); e < end; e += Cfg::kThreads) {
+          const int row = x.row0 + e / kPieces, col = x.n0 + e % kPieces * 4;
+          if (row >= x.row_end || col >= p.n) continue;
+          const uint32_t at = out_stage + part_piece<BN>(e / kPieces, e % kPieces);
+          float4 v[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) v[r] = r < p.split ? ld_cluster_v4(mapa_rank(at, static_cast<uint32_t>(r))) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int r = 1; r < 8; ++r) v[0].x += v[r].x, v[0].y += v[r].y, v[0].z += v[r].z, v[0].w += v[r].w;
+          store_four(p, base + row * p.ldc + col, v[0], p.n - col);
+        }
       }
     }
   }
@@ -737,6 +800,79 @@ cudaError_t launch(const CUtensorMap& mp, const CUtensorMap& mq, const CUtensorM
   return cudaLaunchKernelEx(&cfg, instance<Cfg>(dev), mp, mq, mc, p);
 }
 
+// Clusters of `split` CTAs that the device holds at once (a GPC holds whole clusters only; every kernel here leaves room for one
+// CTA per SM).
+int resident_clusters(int dev, int split, int sms) {
+  static std::mutex mutex;
+  static int known[64][9];   // per device and split, 0 = not asked yet
+  if (split == 1 || dev < 0 || dev >= 64) return sms / split;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (known[dev][split] == 0) {
+    using Cfg = BlockCfg<128, false, kOfRows>;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(split);
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, instance<Cfg>(dev), &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known[dev][split] = n;
+  }
+  return known[dev][split];
+}
+
+struct Choice {
+  bool swap = false, pair = false;
+  int bn = 128, split = 1;
+};
+
+// Which tiles, and how many CTAs share the blocks of one.  Up to 64 rows (of a group: on average): weights on the accumulator's rows
+// and as few columns as hold the rows.  Else the smaller estimate, in cycles, of pairs of CTAs on 256 x 256 and of single
+// ones on 128 x 128.  Measured per block: pairs 700 (1260 where rows and columns have scales of their own), single CTAs 540
+// (640), which is what an SM takes in of operands; around the blocks of a tile 2500 and 1500; 6500 for clusters that add parts up.
+// (4096 wide and deep, pairs / single / with K split: 100 rows 17.8 / 13.5 / 10.1 us, 256 18.0 / 13.9 / 13.0, 1024 20.5 / 26.0.)
+Choice choose(const pmlb_block_gemm_desc& d, int dev, int sms) {
+  const bool by_rows = d.groups > 0 && d.group_dim == PMLB_GROUP_ROWS, by_terms = d.groups > 0 && !by_rows;
+  const int num_kb = (d.k + kBlock - 1) / kBlock, kb = by_terms ? (num_kb + d.groups - 1) / d.groups : num_kb;
+  const int groups = by_rows ? std::min(d.groups, d.m) : 1;   // with rows of their own, at most
+  const int rows = static_cast<int>((static_cast<long long>(d.m) + groups - 1) / groups);
+  // (groups of rows end inside a tile: half a tile each on average)
+  auto tiles = [&](int tile_rows, int tile_cols) {
+    const double high = by_rows ? static_cast<double>(d.m) / tile_rows + 0.5 * groups : std::ceil(static_cast<double>(d.m) / tile_rows);
+    return high * std::ceil(static_cast<double>(d.n) / tile_cols) * (by_terms ? d.groups : 1);
+  };
+  // (a launch with K split has one tile per cluster: the tiles there may be, not those there are on average)
+  auto fits = [&](int tile_rows, int split) {
+    const double high = by_rows ? d.m / tile_rows + groups : std::ceil(static_cast<double>(d.m) / tile_rows);
+    return high * std::ceil(d.n / 128.0) * (by_terms ? d.groups : 1) <= resident_clusters(dev, split, sms);
+  };
+  Choice c;
+  if (rows <= 64) {
+    c.swap = true;
+    c.bn = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+    while (c.split < 8 && kb >= c.split * 4 && fits(c.bn, c.split * 2)) c.split *= 2;
+    return c;
+  }
+  const bool both = d.b_scale_rows == 1;
+  double best = std::ceil(tiles(256, 256) / (sms / 2)) * (kb * (both ? 1260.0 : 700.0) + 2500.0);
+  c.pair = true, c.bn = 256;
+  for (int split = 1; split <= 8 && split <= kb; split *= 2) {
+    if (split > 1 && !fits(128, split)) break;
+    const double waves = split > 1 ? 1.0 : std::ceil(tiles(128, 128) / sms);
+    const double t = waves * ((kb + split - 1) / split * (both ? 640.0 : 540.0) + 1500.0) + (split > 1 ? 6500.0 : 0.0);
+    if (t < best) best = t, c.pair = false, c.bn = 128, c.split = split;
+  }
+  return c;
+}
+
 uint32_t f8_format(int dtype) { return dtype == PMLB_F8E5M2 ? 1u : 0u; }
 
 }  // namespace
@@ -761,12 +897,9 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   p.out_align = bits % 32 == 0 ? 32 : (bits % 16 == 0 ? 16 : 1);
   p.status = status;
 
-  // Rows that a tile of tokens has to hold: those of the product, or of a group on average.
-  const long long rows = by_rows ? (d.m + d.groups - 1) / d.groups : d.m;
-  const bool swap = rows <= 64, pair = !swap && rows > 128;
-  int bn = pair ? 256 : 128;
-  if (swap) bn = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
-  const int ctas = pair ? 2 : 1;
+  const Choice choice = choose(d, dev, sms);
+  const bool swap = choice.swap, pair = choice.pair;
+  const int bn = choice.bn, ctas = pair ? 2 : 1;
   const int tile_rows = swap ? bn : 128 * ctas, tile_cols = swap ? 128 * ctas : bn;
   p.tiles_m = (d.m + tile_rows - 1) / tile_rows;
   p.tiles_n = (d.n + tile_cols - 1) / tile_cols;
@@ -777,10 +910,7 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
     *err = "block_gemm: too many tiles";
     return PMLB_ERR_UNSUPPORTED;
   }
-  p.split = 1;
-  if (swap) {
-    while (p.split < 8 && tiles * p.split * 2 <= sms && p.num_kb >= p.split * 4) p.split *= 2;
-  }
+  p.split = choice.split;
   const int grid = p.split > 1 ? static_cast<int>(tiles) * p.split : static_cast<int>(std::min<long long>(tiles, sms / ctas)) * ctas;
   // bits: [4,6) f32 accumulators, [7,10) and [10,13) formats of the two operands, [17,23) N >> 3, [24,29) M >> 4
   p.idesc = 1u << 4 | f8_format(swap ? d.b_dtype : d.a_dtype) << 7 | f8_format(swap ? d.a_dtype : d.b_dtype) << 10 |

@@ -486,6 +486,11 @@ pmlb_status pmlb_special_invoke(pmlb_plan* plan, void* stream, const void* in0, 
  * lda, ldb and stride_b are multiples of 16 and the operands start on 16 bytes. */
 #define PMLB_GROUP_ROWS 0
 #define PMLB_GROUP_TERMS 1
+/* The library chooses the tiles (0); these force them, for testing one against another: the rows of C on the columns of the
+ * accumulators (meant for few rows), single CTAs on 128 x 128, pairs of CTAs on 256 x 256. */
+#define PMLB_BLOCK_TILES_FEW 1
+#define PMLB_BLOCK_TILES_SINGLE 2
+#define PMLB_BLOCK_TILES_PAIR 3
 
 typedef struct {
   int32_t a_dtype, b_dtype;          /* PMLB_F8E4M3 or PMLB_F8E5M2 */
@@ -495,7 +500,7 @@ typedef struct {
   int64_t lda, ldb, ldc;             /* elements between rows */
   int64_t stride_b, stride_c;        /* elements between the groups' B (ROWS) or C (TERMS) */
   int32_t b_scale_rows;              /* 128 or 1 */
-  int32_t reserved0;
+  int32_t tiles;                     /* 0 = choose, or PMLB_BLOCK_TILES_* */
   int64_t a_scale_row, a_scale_block;/* elements from one row's scale to the next row's / to the next block's */
   int64_t b_scale_row, b_scale_block, b_scale_group; /* row: of 128 rows of B, or of one */
 } pmlb_block_gemm_desc;

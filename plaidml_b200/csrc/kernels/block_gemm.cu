@@ -855,7 +855,7 @@ Choice choose(const pmlb_block_gemm_desc& d, int dev, int sms) {
     return high * std::ceil(d.n / 128.0) * (by_terms ? d.groups : 1) <= resident_clusters(dev, split, sms);
   };
   Choice c;
-  if (rows <= 64) {
+  if (d.tiles == PMLB_BLOCK_TILES_FEW || (d.tiles == 0 && rows <= 64)) {
     c.swap = true;
     c.bn = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
     while (c.split < 8 && kb >= c.split * 4 && fits(c.bn, c.split * 2)) c.split *= 2;
@@ -864,6 +864,8 @@ Choice choose(const pmlb_block_gemm_desc& d, int dev, int sms) {
   const bool both = d.b_scale_rows == 1;
   double best = std::ceil(tiles(256, 256) / (sms / 2)) * (kb * (both ? 1260.0 : 700.0) + 2500.0);
   c.pair = true, c.bn = 256;
+  if (d.tiles == PMLB_BLOCK_TILES_PAIR) return c;
+  if (d.tiles == PMLB_BLOCK_TILES_SINGLE) best = INFINITY;
   for (int split = 1; split <= 8 && split <= kb; split *= 2) {
     if (split > 1 && !fits(128, split)) break;
     const double waves = split > 1 ? 1.0 : std::ceil(tiles(128, 128) / sms);

@@ -49,14 +49,15 @@ struct Elem<__half> {
   static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
 };
 
-// N elements: 16 bytes, or one where rows are not aligned.
+// N elements: 16 bytes, or as many as the rows' alignment allows (then a thread has more places of a row at a time, strips of
+// a block's width apart, so that as much is on its way).
 template <class T, int N>
 struct __align__(sizeof(T) * N) Pack {
   T e[N];
 };
 
 template <class P>
-__device__ __forceinline__ P load_once(const void* at) {   // (read once: no place in L1)
+__device__ __forceinline__ P load_once(const void* at) {   // (whole pieces are read once: no place in L1)
   if constexpr (sizeof(P) == 16) {
     uint4 u;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(at));
@@ -66,50 +67,69 @@ __device__ __forceinline__ P load_once(const void* at) {   // (read once: no pla
   }
 }
 
-// Adds U of the token's rows, from choice j on, to the sums of columns c, c + 1, ..
-template <class T, int N, int U>
-__device__ __forceinline__ void add_rows(const CombineParams& p, const int32_t* position, const float* weights, int j, int c, float (&sum)[N]) {
+template <class T, int N>
+struct Strips {
+  static constexpr int kBytes = N * static_cast<int>(sizeof(T)), value = kBytes >= 16 ? 1 : (kBytes == 8 ? 2 : 4);
+};
+
+// Adds U of the token's rows, from choice j on, to the sums of this thread's columns: N from c on, and N more every `step`.
+template <class T, int N, int S, int U>
+__device__ __forceinline__ void add_rows(const CombineParams& p, const int32_t* position, const float* weights, int j, int c, int step,
+                                         float (&sum)[S][N]) {
   using P = Pack<T, N>;
-  P row[U];
+  P row[U][S];
   float w[U];
   bool there[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int r = __ldg(position + j + u);
     there[u] = static_cast<unsigned>(r) < static_cast<unsigned>(p.rows);
-    row[u] = load_once<P>(static_cast<const T*>(p.y) + (there[u] ? r * p.ldy : 0) + c);
+    const T* y = static_cast<const T*>(p.y) + (there[u] ? r * p.ldy : 0);
+#pragma unroll
+    for (int s = 0; s < S; ++s) row[u][s] = load_once<P>(y + (s == 0 || c + s * step < p.width ? c + s * step : c));
     w[u] = weights != nullptr ? __ldg(weights + j + u) : 1.f;
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float v = fmaf(w[u], Elem<T>::get(row[u].e[e]), sum[e]);
-      sum[e] = there[u] ? v : sum[e];
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = fmaf(w[u], Elem<T>::get(row[u][s].e[e]), sum[s][e]);
+        sum[s][e] = there[u] ? v : sum[s][e];
+      }
     }
   }
 }
 
 template <class T, int N>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const CombineParams p) {
+  constexpr int S = Strips<T, N>::value, kStep = kThreads * N;
   dependent_entry();
   const long long t = blockIdx.x;
   const int32_t* position = p.position + t * p.top_k;
   const float* weights = p.weights != nullptr ? p.weights + t * p.top_k : nullptr;
   T* out = static_cast<T*>(p.out) + t * p.ldo;
-  for (int c = threadIdx.x * N; c < p.width; c += kThreads * N) {
-    float sum[N];
+  for (int c = threadIdx.x * N; c < p.width; c += S * kStep) {
+    float sum[S][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum[e] = 0.f;
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[s][e] = 0.f;
+    }
     int j = p.rows > 0 ? 0 : p.top_k;   // (without rows there is nothing to read, not even row 0)
-    for (; j + 8 <= p.top_k; j += 8) add_rows<T, N, 8>(p, position, weights, j, c, sum);
-    if (j + 4 <= p.top_k) add_rows<T, N, 4>(p, position, weights, j, c, sum), j += 4;
-    if (j + 2 <= p.top_k) add_rows<T, N, 2>(p, position, weights, j, c, sum), j += 2;
-    if (j < p.top_k) add_rows<T, N, 1>(p, position, weights, j, c, sum);
-    Pack<T, N> o;
+    for (; j + 8 <= p.top_k; j += 8) add_rows<T, N, S, 8>(p, position, weights, j, c, kStep, sum);
+    if (j + 4 <= p.top_k) add_rows<T, N, S, 4>(p, position, weights, j, c, kStep, sum), j += 4;
+    if (j + 2 <= p.top_k) add_rows<T, N, S, 2>(p, position, weights, j, c, kStep, sum), j += 2;
+    if (j < p.top_k) add_rows<T, N, S, 1>(p, position, weights, j, c, kStep, sum);
 #pragma unroll
-    for (int e = 0; e < N; ++e) o.e[e] = Elem<T>::put(sum[e]);
-    *reinterpret_cast<Pack<T, N>*>(out + c) = o;
+    for (int s = 0; s < S; ++s) {
+      if (s > 0 && c + s * kStep >= p.width) break;
+      Pack<T, N> o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o.e[e] = Elem<T>::put(sum[s][e]);
+      *reinterpret_cast<Pack<T, N>*>(out + c + s * kStep) = o;
+    }
   }
 }
 
@@ -129,24 +149,34 @@ __device__ __forceinline__ void grad_rows(const CombineParams& p, long long t, i
     dot[u] = 0.f;
   }
   auto there = [&](int u) { return static_cast<unsigned>(at[u]) < static_cast<unsigned>(p.rows); };
-  for (int c = threadIdx.x * N; c < p.width; c += kGradThreads * N) {
-    P row[U];
-    const P g = load_once<P>(dout + c);
-    if (dots) {
+  constexpr int S = Strips<T, N>::value, kStep = kGradThreads * N;
+  for (int c0 = threadIdx.x * N; c0 < p.width; c0 += S * kStep) {
+    P row[U][S], g[S];
 #pragma unroll
-      for (int u = 0; u < U; ++u) row[u] = load_once<P>(static_cast<const T*>(p.y) + (there(u) ? at[u] * p.ldy : 0) + c);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int s = 0; s < S; ++s) {
+      const int c = s == 0 || c0 + s * kStep < p.width ? c0 + s * kStep : c0;
+      g[s] = load_once<P>(dout + c);
       if (dots) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) dot[u] = fmaf(Elem<T>::get(g.e[e]), Elem<T>::get(row[u].e[e]), dot[u]);
+        for (int u = 0; u < U; ++u) row[u][s] = load_once<P>(static_cast<const T*>(p.y) + (there(u) ? at[u] * p.ldy : 0) + c);
       }
-      if (p.dy != nullptr && there(u)) {
-        P o;
+    }
 #pragma unroll
-        for (int e = 0; e < N; ++e) o.e[e] = Elem<T>::put(w[u] * Elem<T>::get(g.e[e]));
-        *reinterpret_cast<P*>(static_cast<T*>(p.dy) + at[u] * p.ldy + c) = o;
+    for (int s = 0; s < S; ++s) {
+      const int c = c0 + s * kStep;
+      if (s > 0 && c >= p.width) break;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (dots) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) dot[u] = fmaf(Elem<T>::get(g[s].e[e]), Elem<T>::get(row[u][s].e[e]), dot[u]);
+        }
+        if (p.dy != nullptr && there(u)) {
+          P o;
+#pragma unroll
+          for (int e = 0; e < N; ++e) o.e[e] = Elem<T>::put(w[u] * Elem<T>::get(g[s].e[e]));
+          *reinterpret_cast<P*>(static_cast<T*>(p.dy) + at[u] * p.ldy + c) = o;
+        }
       }
     }
   }
@@ -201,19 +231,25 @@ __global__ void __launch_bounds__(kGradThreads) combine_grad_kernel(const Combin
   if (j < p.top_k) grad_rows<T, N, 1>(p, t, j, part);
 }
 
-template <class T>
-cudaError_t launch_typed(CombineParams p, bool grad, cudaStream_t stream) {
-  constexpr int kWide = 16 / sizeof(T);
-  auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
-  const bool wide = p.width % kWide == 0 && p.ldy % kWide == 0 && p.ldo % kWide == 0 && aligned(p.y) && aligned(p.dout) && aligned(p.out) &&
-                    aligned(p.dy);
-  if (!grad) {
-    return launch_dependent(wide ? combine_kernel<T, kWide> : combine_kernel<T, 1>, dim3(static_cast<unsigned>(p.tokens)), kThreads, stream, p);
-  }
+template <class T, int N>
+cudaError_t launch_sized(CombineParams p, bool grad, cudaStream_t stream) {
+  if (!grad) return launch_dependent(combine_kernel<T, N>, dim3(static_cast<unsigned>(p.tokens)), kThreads, stream, p);
   constexpr int kRows = kGradThreads / 32 * kRowsPerWarp;
   p.row_blocks = p.dy != nullptr ? (p.rows + kRows - 1) / kRows : 0;
-  const dim3 grid(static_cast<unsigned>(p.row_blocks + p.tokens));
-  return launch_dependent(wide ? combine_grad_kernel<T, kWide> : combine_grad_kernel<T, 1>, grid, kGradThreads, stream, p);
+  return launch_dependent(combine_grad_kernel<T, N>, dim3(static_cast<unsigned>(p.row_blocks + p.tokens)), kGradThreads, stream, p);
+}
+
+template <class T>
+cudaError_t launch_typed(const CombineParams& p, bool grad, cudaStream_t stream) {
+  // bytes that every row starts on and is made of
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.out) |
+                         reinterpret_cast<uintptr_t>(p.dy) | static_cast<uintptr_t>((p.width | p.ldy | p.ldo) * sizeof(T));
+  if (bits % 16 == 0) return launch_sized<T, 16 / sizeof(T)>(p, grad, stream);
+  if (bits % 8 == 0) return launch_sized<T, 8 / sizeof(T)>(p, grad, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (bits % 4 == 0) return launch_sized<T, 2>(p, grad, stream);
+  }
+  return launch_sized<T, 1>(p, grad, stream);
 }
 
 cudaError_t launch_of(int dtype, const CombineParams& p, bool grad, cudaStream_t stream) {

@@ -1539,6 +1539,7 @@ std::string block_gemm_problem(const pmlb_block_gemm_desc& d) {
   if (d.m > (1 << 30) || d.n > (1 << 30) || d.k > (1 << 30)) return "block_gemm: sizes above 2^30";
   if (d.groups < 0 || d.groups > 1024) return "block_gemm: groups must be 0..1024";
   if (d.groups > 0 && d.group_dim != PMLB_GROUP_ROWS && d.group_dim != PMLB_GROUP_TERMS) return "block_gemm: unknown group dimension";
+  if (d.tiles < 0 || d.tiles > PMLB_BLOCK_TILES_PAIR) return "block_gemm: unknown tiles";
   if (d.b_scale_rows != 128 && d.b_scale_rows != 1) return "block_gemm: B has a scale for each 128 rows or for each row";
   if (d.lda < d.k || d.ldb < d.k || d.ldc < d.n) return "block_gemm: a row stride smaller than a row";
   if (d.lda % 16 != 0 || d.ldb % 16 != 0) return "block_gemm: lda and ldb must be multiples of 16";

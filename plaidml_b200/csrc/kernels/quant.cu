@@ -41,6 +41,21 @@ struct Eight {
     if (n >= 8 && vec) {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(In) / 2); ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    } else if (sizeof(In) == 2 && n >= 8) {
+      // rows that start anywhere: words, between two halves where the first one is not aligned
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+      uint32_t w[4];
+      if (reinterpret_cast<uintptr_t>(src) % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(h) + i);
+      } else {
+        const uint32_t *mid = reinterpret_cast<const uint32_t*>(h + 1), a = __ldg(mid), b = __ldg(mid + 1), c = __ldg(mid + 2);
+        w[0] = __ldg(h) | a << 16;
+        w[1] = a >> 16 | b << 16;
+        w[2] = b >> 16 | c << 16;
+        w[3] = c >> 16 | static_cast<uint32_t>(__ldg(h + 7)) << 16;
+      }
+      raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
       In v[8];
 #pragma unroll
@@ -290,7 +305,7 @@ __global__ void __launch_bounds__(COLUMNS ? 256 : 512) quant_tile_kernel(const Q
 template <class In, bool E5M2>
 cudaError_t launch_typed(const pmlb_quant_desc& d, const QuantParams& p, cudaStream_t stream) {
   if (d.form == PMLB_QUANT_ROWS) {
-    // loads at once: four, or what a short row has
+    // loads at once: four, or what a short row has (8192 x 4096 bf16: 20.5 us with four, 22.6 with eight)
     const unsigned x = static_cast<unsigned>((static_cast<long long>(p.rows) + kRowWarps - 1) / kRowWarps);
     if (p.cols > 512) return launch_dependent(quant_rows_kernel<In, E5M2, 4>, dim3(x, (p.cols + 1023) / 1024, d.batch), kRowWarps * 32, stream, p);
     if (p.cols > 256) return launch_dependent(quant_rows_kernel<In, E5M2, 2>, dim3(x, 1, d.batch), kRowWarps * 32, stream, p);

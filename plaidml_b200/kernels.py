@@ -36,6 +36,7 @@ CONV_NO_COLUMN_MERGE = 32
 CONV_MAX_POOL_3X3_S2 = 64
 SPECIAL_GATHER, SPECIAL_SCATTER, SPECIAL_ARGSORT, SPECIAL_PRNG = range(4)
 GROUP_ROWS, GROUP_TERMS = range(2)
+BLOCK_TILES_FEW, BLOCK_TILES_SINGLE, BLOCK_TILES_PAIR = 1, 2, 3
 QUANT_ROWS, QUANT_COLUMNS, QUANT_TILES, QUANT_TILES_TRANSPOSED = range(4)
 ROUTE_SOFTMAX, ROUTE_SIGMOID = range(2)
 OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT = range(5)
@@ -123,7 +124,7 @@ class BlockGemmDesc(C.Structure):
         ("a_dtype", C.c_int32), ("b_dtype", C.c_int32), ("out_dtype", C.c_int32),
         ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("groups", C.c_int32), ("group_dim", C.c_int32),
         ("lda", C.c_int64), ("ldb", C.c_int64), ("ldc", C.c_int64), ("stride_b", C.c_int64), ("stride_c", C.c_int64),
-        ("b_scale_rows", C.c_int32), ("reserved0", C.c_int32),
+        ("b_scale_rows", C.c_int32), ("tiles", C.c_int32),
         ("a_scale_row", C.c_int64), ("a_scale_block", C.c_int64),
         ("b_scale_row", C.c_int64), ("b_scale_block", C.c_int64), ("b_scale_group", C.c_int64),
     ]
@@ -329,13 +330,13 @@ def _blocks(n: int) -> int:
 
 def block_gemm_desc(a_dtype: int, b_dtype: int, out_dtype: int, m: int, n: int, k: int, lda=None, ldb=None, ldc=None,
                     groups: int = 0, group_dim: int = GROUP_ROWS, stride_b=None, stride_c=None, b_scale_rows: int = 128,
-                    a_scale_row=None, a_scale_block=None, b_scale_row=None, b_scale_block=None,
-                    b_scale_group=None) -> BlockGemmDesc:
+                    a_scale_row=None, a_scale_block=None, b_scale_row=None, b_scale_block=None, b_scale_group=None,
+                    tiles: int = 0) -> BlockGemmDesc:
     """Defaults: dense matrices and groups; the scales of A as [blocks][m], those of B as [n / 128][blocks]
     (b_scale_rows = 128) or [blocks][n] (b_scale_rows = 1)."""
     d = BlockGemmDesc()
     d.a_dtype, d.b_dtype, d.out_dtype, d.m, d.n, d.k = a_dtype, b_dtype, out_dtype, m, n, k
-    d.groups, d.group_dim, d.b_scale_rows = groups, group_dim, b_scale_rows
+    d.groups, d.group_dim, d.b_scale_rows, d.tiles = groups, group_dim, b_scale_rows, tiles
     d.lda, d.ldb, d.ldc = (k if lda is None else lda), (k if ldb is None else ldb), (n if ldc is None else ldc)
     d.stride_b = n * d.ldb if stride_b is None else stride_b
     d.stride_c = m * d.ldc if stride_c is None else stride_c

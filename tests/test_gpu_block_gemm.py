@@ -127,22 +127,53 @@ def test_product_strides(m, out, ldc):
     assert (c[:m, n:] == 7).all() and (c[m] == 7).all()
 
 
+TILES = [K.BLOCK_TILES_FEW, K.BLOCK_TILES_SINGLE, K.BLOCK_TILES_PAIR]
+
+
+@pytest.mark.parametrize("tiles", TILES)
+@pytest.mark.parametrize("out", [K.BF16, K.F32])
+@pytest.mark.parametrize("b_rows", [1, 128])
+@pytest.mark.parametrize("m, n, k", [(1, 130, 128), (127, 257, 140), (300, 515, 3000), (257, 1000, 1030), (1030, 264, 96), (520, 2051, 257)])
+def test_product_by_each_kind_of_tiles(m, n, k, b_rows, out, tiles):
+    x = make(m, n, k, b_rows=b_rows, seed=m + n)
+    c = torch.full((m + 1, n + 5), 7.0, dtype=TORCH_OF[out], device="cuda")
+    plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, out, m, n, k, lda=x["ld"], ldb=x["ld"], ldc=n + 5, b_scale_rows=b_rows, tiles=tiles))
+    run(plan, x, c)
+    plan.check()
+    check(c[:m, :n], *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], b_rows), k, out)
+    assert (c[m] == 7).all() and (c[:, n:] == 7).all()
+
+
+def test_products_with_k_split_by_any_number_of_ctas():
+    """Few tiles and a deep K: the split follows the shape; each is compared with the formula and is the same on every call."""
+    for m, n, k in ((20, 128, 4096), (1, 1000, 8192), (128, 128, 8000), (100, 500, 4096), (256, 1024, 8192), (130, 2048, 2048)):
+        x = make(m, n, k, seed=k)
+        c, again = (torch.empty((m, n), dtype=torch.float32, device="cuda") for _ in range(2))
+        plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.F32, m, n, k))
+        run(plan, x, c)
+        run(plan, x, again)
+        plan.check()
+        check(c, *expect(x["a"], x["sa"], x["b"], x["sb"], 128), k, K.F32)
+        assert torch.equal(c, again)
+
+
 GROUPS = {
     "one": [5], "empty": [0, 0, 0], "gaps": [0, 3, 0, 0, 130, 1, 0, 17, 0], "even": [64] * 6, "tails": [1, 127, 128, 129, 255, 256, 257, 0],
     "many": [(7 * i) % 5 for i in range(257)], "long": [700, 0, 900, 2],
 }
 
 
+@pytest.mark.parametrize("tiles", [0] + TILES)
 @pytest.mark.parametrize("out", [K.BF16, K.F32])
 @pytest.mark.parametrize("name", GROUPS)
-def test_groups_of_rows(name, out):
+def test_groups_of_rows(name, out, tiles):
     counts = GROUPS[name]
     groups, used, n, k = len(counts), sum(counts), 264, 400
     m = used + 9                                    # rows behind the last group
     x = make(m, n, k, each=(groups,), seed=len(name))
     offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
     c = torch.full((m, n), 3.0, dtype=TORCH_OF[out], device="cuda")
-    plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, out, m, n, k, lda=x["ld"], ldb=x["ld"], groups=groups))
+    plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, out, m, n, k, lda=x["ld"], ldb=x["ld"], groups=groups, tiles=tiles))
     run(plan, x, c, offsets)
     plan.check()
     at = 0
@@ -156,13 +187,14 @@ def test_groups_of_rows(name, out):
 
 @pytest.mark.parametrize("counts", [[1, 2, 0, 3], [0, 0], [5], [2, 0, 0, 1, 30, 0, 4]])
 @pytest.mark.parametrize("m, n", [(1, 200), (100, 300), (500, 129)])
-def test_groups_of_terms(counts, m, n):
+@pytest.mark.parametrize("tiles", [0] + TILES)
+def test_groups_of_terms(counts, m, n, tiles):
     groups, k = len(counts), max(1, 128 * sum(counts))
     x = make(m, n, k, b_rows=1, seed=m + groups)
     offsets = (torch.tensor([0] + counts).cumsum(0) * 128).int().cuda()
     c = torch.full((groups, m, n + 3), 3.0, dtype=torch.float32, device="cuda")
     plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.F32, m, n, k, lda=x["ld"], ldb=x["ld"], ldc=n + 3, groups=groups,
-                                                  group_dim=K.GROUP_TERMS, b_scale_rows=1))
+                                                  group_dim=K.GROUP_TERMS, b_scale_rows=1, tiles=tiles))
     run(plan, x, c, offsets)
     plan.check()
     for g in range(groups):
@@ -204,7 +236,7 @@ def test_a_nan_and_an_infinity_stay_in_their_rows_and_columns(m):
     check(c[fine], want[fine], size[fine], k, K.F32)
 
 
-@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("m", [3, 300, 5000])
 def test_calls_are_alike_on_streams_and_in_graphs(m):
     """One plan on two streams at once, captured and replayed with other inputs in the same place: bits of the plain call."""
     n, k = 512, 2048

@@ -35,7 +35,7 @@ def product(**fields):
     (dict(groups=4, group_dim=2), "dimension"), (dict(groups=4, stride_b=200 * 256 + 8), "multiple of 16"),
     (dict(groups=4, stride_b=256), "overlap"), (dict(groups=4, group_dim=K.GROUP_TERMS, stride_c=200), "overlap"),
     (dict(b_scale_rows=64), "scale"), (dict(a_scale_row=-1), "negative"), (dict(b_scale_group=-4), "negative"),
-    (dict(m=(1 << 30) + 1), "2^30"),
+    (dict(m=(1 << 30) + 1), "2^30"), (dict(tiles=4), "tiles"), (dict(tiles=-1), "tiles"),
 ])
 def test_products_that_are_refused(fields, word):
     assert word in problem("block_gemm", product(**fields))

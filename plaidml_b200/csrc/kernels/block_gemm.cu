@@ -6,6 +6,13 @@
 // The scales differ from block to block, so a block's products get a TMEM accumulator of their own, and eight warps that hold
 // the tile's sums in registers add  sum += scale * accumulator  (packed f32 multiply-adds), while the tensor core works on the
 // next block in another accumulator.  The tensor core thus never adds more than 128 terms, and the sums are f32.
+//
+// What bounds it.  Large products (CTA pairs on 256 x 256 tiles): a block's MMAs take 512 cycles, a block 700.  Two accumulators of
+// 256 columns fill TMEM, and one's way round -- MMAs 512, their completion to both CTAs some 200, half of the sums' loads
+// and additions before it can be handed back 330, that to the issuer and its first MMA 350 -- is 1400 for two blocks.  (Found
+// with clock readings in a copy: the issuer waits for an accumulator in 62 of 64 blocks and for operands in 1; without the
+// additions a block takes 620, with half of the MMAs 600.)  Around it, a tile's results cost 2000 cycles of which the two
+// accumulators hide 1400.  Few rows: the weights' bytes from HBM (5.3 to 6.4 TB/s of them).
 #include "block_gemm.h"
 
 #include <cuda.h>
@@ -17,6 +24,7 @@
 #include <cmath>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "dependent_launch.h"
 #include "ptx.cuh"
@@ -59,6 +67,7 @@ struct BlockCfg {
   static constexpr int kStages = std::min(10, (232448 - 1024 - kPartBytes - kScaleBytes - kStageOutBytes - kTailBytes) / kStageBytes);
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kPartBytes + kScaleBytes + kStageOutBytes + kTailBytes;
   static_assert(kStages >= 3 && kSmem <= 232448, "shared memory");
+  static_assert(kSwap || kCols == 64 || kCols == 128, "boxes");
   static_assert(kSwap || !kSplits || kStageOutBytes >= BN * 128 * 4, "room for a part");
 };
 
@@ -98,7 +107,7 @@ __device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) { asm 
 
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  asm volatile("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 
@@ -202,6 +211,18 @@ __device__ __forceinline__ uint32_t part_piece(uint32_t row, uint32_t piece) { r
 // Results leave through shared memory in boxes of 32 rows of 128 bytes (64 columns of 16 bits, or 32 of 32 bits), in the layout
 // of a TMA store with 128-byte swizzle: 16-byte pieces permuted by the row, which spreads a lane's row over the banks.
 __device__ __forceinline__ uint32_t box_piece(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }
+
+// Eight sums as 16-bit values.
+template <bool BF16>
+__device__ __forceinline__ uint4 pack_eight(const uint64_t* sum) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = unpack2(sum[i]);
+    u[i] = cvt_pack16<BF16, false>(v.x, v.y);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
 
 // A box by plain stores: rows [0, rows) of C from element `base` on, `n` columns of which exist.
 __device__ __forceinline__ void store_box(const BlockGemmParams& p, uint32_t at, long long base, int rows, int n, int lane) {
@@ -539,8 +560,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     constexpr int kCols = Cfg::kCols;
     const int quarter = warp & 3, first_col = (w >> 2) * kCols;   // TMEM lanes [32 quarter, ...), columns [first_col, ...)
     // Columns loaded from TMEM at a time.  Two warps take turns on a scheduler, so one set of registers is enough; what counts is
-    // that the compiler finds them beside the sums without moving any (4096^3: 16 at a time 70 us, 32 76, 64 68; two sets
-    // of 32 73; a weight gradient's two scales per element: 100, 107, 120).
+    // that the compiler finds them beside the sums without moving any (4096^3, bf16: 64 at a time 64.8 us, 16 67.1, 32 74.6; with
+    // scales of rows and columns 16 at a time 89, 32 95, 64 95, and 100 where the two scales are multiplied first).
     constexpr int kChunk = kCols < 16 ? kCols : (SCALES == kOfRows && kCols >= 64 ? 64 : 16), kChunks = kCols / kChunk;
     const uint32_t t_mine = tmem_base + static_cast<uint32_t>(first_col) + (static_cast<uint32_t>(quarter * 32) << 16);
     int acc = 0, slot = 0, stage = 0;
@@ -589,13 +610,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       auto add = [&](uint32_t (&v)[kChunk], int c) {
 #pragma unroll
         for (int e = 0; e < kChunk; e += 4) {
-          uint64_t s0 = row2, s1 = row2;
+          uint64_t v0 = pack2(v[e], v[e + 1]), v1 = pack2(v[e + 2], v[e + 3]);
           if constexpr (SCALES != kOfRows) {
             const uint4 u = ld_shared_v4(scales + (c + e) * 4);
-            s0 = mul2(pack2(u.x, u.y), row2), s1 = mul2(pack2(u.z, u.w), row2);
+            v0 = mul2(v0, pack2(u.x, u.y)), v1 = mul2(v1, pack2(u.z, u.w));
           }
-          fma2(sum[(c + e) / 2], pack2(v[e], v[e + 1]), s0);
-          fma2(sum[(c + e) / 2 + 1], pack2(v[e + 2], v[e + 3]), s1);
+          fma2(sum[(c + e) / 2], v0, row2);
+          fma2(sum[(c + e) / 2 + 1], v1, row2);
         }
       };
       for (int kb = x.kb0; kb < x.kb1 && ok; ++kb) {
@@ -644,54 +665,59 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         // warp itself, they held it up for 2 us per tile: no MMAs in that time, as both accumulators were full).
         const int row = x.row0 + side * 128 + quarter * 32, col = x.n0 + first_col;
         const int rows = min(x.row_end - row, 32);
-        const uint32_t at = out_stage + static_cast<uint32_t>(w) * 8192u;
-        const bool f32 = p.out_dtype == PMLB_F32;
-        // (a box that holds rows of the next group is stored row by row)
-        const bool by_tma = p.out_align >= 16 && (rows == 32 || x.row_end == p.m);
         if (rows > 0) {
+          const uint32_t places = out_stage + static_cast<uint32_t>(w) * 8192u;
+          // (a box that holds rows of the next group is stored row by row)
+          const bool by_tma = p.out_align >= 16 && (rows == 32 || x.row_end == p.m);
+          // 16 bits: the warp's boxes of 64 columns together, one fence and one group of copies.  f32: boxes of 32 columns one
+          // after the other, in the two places by turns, the next written while the last one leaves.
+          auto leave = [&](auto wide_tag, auto first_tag, auto pack) {
+            constexpr int kWide = decltype(wide_tag)::value, kFirst = decltype(first_tag)::value;
+            constexpr int kBoxes = kWide == 32 ? 1 : kCols / kWide;
+            const uint32_t at = places + (kFirst & 1) * 4096u;
+            if (lane == 0) bulk_wait_group_read<kWide == 32 ? 1 : 0>();
+            __syncwarp();
+            const uint32_t mine = at + box_piece(lane, 0);
 #pragma unroll
-          for (int j = 0; j < kCols; j += 16) {
-            const int box = f32 ? j / 32 : j / 64;          // (two boxes of staging: f32 goes round it twice)
-            const uint32_t to = at + static_cast<uint32_t>(box & 1) * 4096u;
-            if (j % 64 == 0 && (j == 0 || f32)) {
-              if (lane == 0) bulk_wait_group_read<0>();
-              __syncwarp();
+            for (int b = 0; b < kBoxes; ++b) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) st_shared_v4((mine ^ (q << 4)) + b * 4096, pack((kFirst + b) * kWide + q * (kWide / 8)));
             }
-            uint32_t u[16];
-            float v[16];
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float2 t = unpack2(sum[(j + e) / 2]);
-              v[e] = t.x, v[e + 1] = t.y;
-            }
-            if (f32) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(v[e]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) st_shared_v4(to + box_piece(lane, j % 32 / 4 + e), make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]));
+            // (a TMA store writes whole 16-byte units: a row that ends inside one would lose what lies behind it)
+            const int c0 = col + kFirst * kWide;
+            const bool whole = c0 + kBoxes * kWide <= p.n || p.n % (kWide / 8) == 0;
+            if (by_tma && whole) fence_proxy_async_smem();
+            __syncwarp();
+            if (by_tma && whole) {
+              if (lane == 0) {
+                if (c0 < p.n) tma_store_3d(&map_c, at, c0, row, p.terms ? x.group : 0);
+                if (kBoxes == 2 && c0 + kWide < p.n) tma_store_3d(&map_c, at + 4096, c0 + kWide, row, p.terms ? x.group : 0);
+                bulk_commit_group();
+              }
             } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) u[e] = p.out_dtype == PMLB_BF16 ? cvt_pack16<true, false>(v[2 * e], v[2 * e + 1]) : cvt_pack16<false, false>(v[2 * e], v[2 * e + 1]);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) st_shared_v4(to + box_piece(lane, j % 64 / 8 + e), make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]));
-            }
-            if (f32 ? j % 32 == 16 : j % 64 == 48) {
-              const int c0 = col + (f32 ? j - 16 : j - 48);   // the box's first column
-              if (c0 < p.n) {
-                // (a TMA store writes whole 16-byte units: a row that ends inside one would lose what lies behind it)
-                if (by_tma && (c0 + (f32 ? 32 : 64) <= p.n || p.n % (f32 ? 4 : 8) == 0)) {
-                  fence_proxy_async_smem();
-                  __syncwarp();
-                  if (lane == 0) {
-                    tma_store_3d(&map_c, to, c0, row, p.terms ? x.group : 0);
-                    bulk_commit_group();
-                  }
-                } else {
-                  __syncwarp();
-                  store_box(p, to, (p.terms ? x.group * p.stride_c : 0) + row * p.ldc + c0, rows, p.n - c0, lane);
-                }
+#pragma unroll 1
+              for (int b = 0; b < kBoxes; ++b) {
+                const int c = c0 + b * kWide;
+                if (c < p.n) store_box(p, at + b * 4096, (p.terms ? x.group * p.stride_c : 0) + row * p.ldc + c, rows, p.n - c, lane);
               }
             }
+          };
+          using std::integral_constant;
+          if (p.out_dtype == PMLB_F32) {
+            auto pack = [&](int j) {
+              const float2 u = unpack2(sum[j / 2]), v = unpack2(sum[j / 2 + 1]);
+              return make_uint4(__float_as_uint(u.x), __float_as_uint(u.y), __float_as_uint(v.x), __float_as_uint(v.y));
+            };
+            leave(integral_constant<int, 32>(), integral_constant<int, 0>(), pack);
+            leave(integral_constant<int, 32>(), integral_constant<int, 1>(), pack);
+            if constexpr (kCols > 64) {
+              leave(integral_constant<int, 32>(), integral_constant<int, 2>(), pack);
+              leave(integral_constant<int, 32>(), integral_constant<int, 3>(), pack);
+            }
+          } else if (p.out_dtype == PMLB_BF16) {
+            leave(integral_constant<int, 64>(), integral_constant<int, 0>(), [&](int j) { return pack_eight<true>(&sum[j / 2]); });
+          } else {
+            leave(integral_constant<int, 64>(), integral_constant<int, 0>(), [&](int j) { return pack_eight<false>(&sum[j / 2]); });
           }
         }
       }
@@ -836,7 +862,7 @@ struct Choice {
 
 // Which tiles, and how many CTAs share the blocks of one.  Up to 64 rows (of a group: on average): weights on the accumulator's rows
 // and as few columns as hold the rows.  Else the smaller estimate, in cycles, of pairs of CTAs on 256 x 256 and of single
-// ones on 128 x 128.  Measured per block: pairs 700 (1260 where rows and columns have scales of their own), single CTAs 540
+// ones on 128 x 128.  Measured per block: pairs 700 (1150 where rows and columns have scales of their own), single CTAs 540
 // (640), which is what an SM takes in of operands; around the blocks of a tile 2500 and 1500; 6500 for clusters that add parts up.
 // (4096 wide and deep, pairs / single / with K split: 100 rows 17.8 / 13.5 / 10.1 us, 256 18.0 / 13.9 / 13.0, 1024 20.5 / 26.0.)
 Choice choose(const pmlb_block_gemm_desc& d, int dev, int sms) {
@@ -862,7 +888,7 @@ Choice choose(const pmlb_block_gemm_desc& d, int dev, int sms) {
     return c;
   }
   const bool both = d.b_scale_rows == 1;
-  double best = std::ceil(tiles(256, 256) / (sms / 2)) * (kb * (both ? 1260.0 : 700.0) + 2500.0);
+  double best = std::ceil(tiles(256, 256) / (sms / 2)) * (kb * (both ? 1150.0 : 700.0) + 2500.0);
   c.pair = true, c.bn = 256;
   if (d.tiles == PMLB_BLOCK_TILES_PAIR) return c;
   if (d.tiles == PMLB_BLOCK_TILES_SINGLE) best = INFINITY;

@@ -475,8 +475,8 @@ pmlb_status pmlb_special_invoke(pmlb_plan* plan, void* stream, const void* in0, 
  * rows is shared by up to eight CTAs, which adds 2..8 runs of blocks in a fixed order: results are the same on every call.
  *
  * groups = 0: one product.  groups = 1..1024 with `offsets`, int32[groups + 1] in device memory, ascending from 0:
- *   PMLB_GROUP_ROWS   rows [offsets[g], offsets[g + 1]) of A and C belong to B[g] (stride_b elements apart, scales
- *                     b_scale_group apart): the experts' products.  m is the number of rows that A and C have; rows from
+ *   PMLB_GROUP_ROWS   rows [offsets[g], offsets[g + 1]) of A and C belong to B[g] (stride_b elements apart, 0 = one B for
+ *                     all; scales b_scale_group apart): the experts' products.  m is the number of rows that A and C have; rows from
  *                     offsets[groups] on are neither computed nor written.
  *   PMLB_GROUP_TERMS  C[g] (stride_c elements apart) is the product over the terms [offsets[g], offsets[g + 1]) alone:
  *                     the experts' weight gradients, both operands transposed by PMLB_QUANT_COLUMNS.  Offsets are

@@ -79,6 +79,7 @@ struct BlockGemmParams {
   const float *a_scale, *b_scale;
   long long as_row, as_block, bs_row, bs_block, bs_group;
   int b_shift;             // rows of B per scale, as a power of two
+  int b_step;              // 1, or 0 where all groups share one B
   void* out;
   long long ldc, stride_c;
   int out_dtype, out_align;   // bytes that every row and the matrix start on: 32, 16, or less
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
       for (int t = first; t < total && ok; t += units) {
         const Tile x = tile_at(t);
         const int py = (SWAP ? x.n0 : x.row0) + side * 128, qy = (SWAP ? x.row0 : x.n0) + side * (BN / CTAS);
-        const int z = p.terms ? 0 : x.group;
+        const int z = p.terms ? 0 : x.group * p.b_step;
         for (int kb = x.kb0; kb < x.kb1; ++kb) {
           if (!mbar_wait_warp(done_bar(stage), phase ^ 1u, abort_flag)) {
             if (leader && abort_flag[1] == 0) abort_flag[1] = 1;
@@ -919,6 +920,7 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   p.as_row = d.a_scale_row, p.as_block = d.a_scale_block;
   p.bs_row = d.b_scale_row, p.bs_block = d.b_scale_block, p.bs_group = d.b_scale_group;
   p.b_shift = d.b_scale_rows == 128 ? 7 : 0;
+  p.b_step = by_rows && d.stride_b == 0 ? 0 : 1;
   p.out = c, p.ldc = d.ldc, p.stride_c = d.stride_c, p.out_dtype = d.out_dtype;
   const long long ob = d.out_dtype == PMLB_F32 ? 4 : 2;
   const long long bits = static_cast<long long>(reinterpret_cast<uintptr_t>(c)) | (d.ldc * ob) | (by_terms ? d.stride_c * ob : 0);
@@ -949,7 +951,8 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   // (a CTA of a pair fetches 128 rows of one operand and its half of the other)
   const int box_a = tile_rows / ctas, box_b = tile_cols / ctas;
   if (!tc_encode_bytes(&ma, a, d.k, d.m, 1, d.lda, 16, box_a, err)) return PMLB_ERR_INVALID;
-  if (!tc_encode_bytes(&mb, b, d.k, d.n, by_rows ? d.groups : 1, d.ldb, by_rows ? d.stride_b : 16, box_b, err)) return PMLB_ERR_INVALID;
+  const bool many_b = by_rows && d.stride_b != 0;
+  if (!tc_encode_bytes(&mb, b, d.k, d.n, many_b ? d.groups : 1, d.ldb, many_b ? d.stride_b : 16, box_b, err)) return PMLB_ERR_INVALID;
   if (!swap && p.out_align >= 16 &&
       !tc_encode_boxes(&mc, d.out_dtype, c, d.n, d.m, by_terms ? d.groups : 1, d.ldc, by_terms ? d.stride_c : 8, err)) {
     return PMLB_ERR_INVALID;

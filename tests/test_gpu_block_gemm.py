@@ -207,6 +207,19 @@ def test_groups_of_terms(counts, m, n, tiles):
     assert (c[:, :, n:] == 3).all()
 
 
+@pytest.mark.parametrize("tiles", TILES)
+def test_groups_that_share_one_b(tiles):
+    m, n, k, counts = 210, 136, 300, [3, 150, 0, 57]
+    x = make(m, n, k, seed=3)
+    offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    c = torch.empty((m, n), dtype=torch.float32, device="cuda")
+    d = K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.F32, m, n, k, lda=x["ld"], ldb=x["ld"], groups=4, stride_b=0, b_scale_group=0, tiles=tiles)
+    plan = K.Plan("block_gemm", d)
+    run(plan, x, c, offsets)
+    plan.check()
+    check(c, *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], 128), k, K.F32)
+
+
 def test_offsets_outside_the_rows_are_taken_as_the_edge():
     m, n, k = 40, 130, 256
     x = make(m, n, k, each=(4,), seed=2)

@@ -284,6 +284,14 @@ def test_order(tokens, experts, top_k, align):
     check_order(ids, experts, align, spare=align * 2 + 5)
 
 
+@pytest.mark.parametrize("experts, top_k", [(64, 8), (700, 6)])
+def test_order_of_more_pairs_than_fit_in_registers(experts, top_k):
+    g = np.random.Generator(np.random.PCG64(experts))
+    ids = g.integers(-1, experts, (60000, top_k))
+    check_order(ids, experts, 1)
+    check_order(ids, experts, 128, spare=77)
+
+
 @pytest.mark.parametrize("tokens", [10, 5000])
 def test_order_of_a_padded_batch(tokens):
     """Pairs without an expert have no row; all of one expert; none at all."""

@@ -66,7 +66,7 @@ struct BlockCfg {
   static constexpr int kTailBytes = 512 + 2 * (kMaxGroups + 4) * 4;
   static constexpr int kStages = std::min(10, (232448 - 1024 - kPartBytes - kScaleBytes - kStageOutBytes - kTailBytes) / kStageBytes);
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kPartBytes + kScaleBytes + kStageOutBytes + kTailBytes;
-  static_assert(kStages >= 3 && kSmem <= 232448, "shared memory");
+  static_assert(kStages >= kAccs && kStages >= 3 && kSmem <= 232448, "shared memory");   // (kAccs: see the warp that fetches scales)
   static_assert(kSwap || kCols == 64 || kCols == 128, "boxes");
   static_assert(kSwap || !kSplits || kStageOutBytes >= BN * 128 * 4, "room for a part");
 };
@@ -480,9 +480,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
     } else if (warp == 2) {
       // ------------------------------------------------------------ scales
       // Asynchronous copies, kAhead blocks ahead and across tiles: fetched by the warps that use them, scales cost those a trip to
-      // L2 or HBM per block (78 us of a product of 4096^3 were then 15 us of waiting for scales).  A block's products are announced
-      // by the tensor core and by this warp.  Step s waits for the products of block s - kAccs: they were begun after all of block
-      // s - 2 kAccs had been read, so the slots up to block s - 2 kAccs - 1 are free.
+      // L2 or HBM per block (a weight gradient of 4096 x 2048 x 8190: 152 us that way, 113 so).  A block's products are announced by
+      // the tensor core and by this warp.  Step s waits for the products of block s - kAccs: they were begun after all of block
+      // s - 2 kAccs - 1 had been added, so that its slot and those before it are free.
       constexpr int kRowCopies = 4, kColCopies = SCALES == kOfRows ? 1 : (BN + 31) / 32;
       int ahead_t = first, ahead_kb = 0, ahead_end = 0, to = 0;
       const float *row_from[kRowCopies], *col_from[kColCopies];

@@ -683,7 +683,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
           // (a box that holds rows of the next group is stored row by row)
           const bool by_tma = p.out_align >= 16 && (rows == 32 || x.row_end == p.m);
           // 16 bits: the warp's boxes of 64 columns together, one fence and one group of copies.  f32: boxes of 32 columns one
-          // after the other, in the two places by turns, the next written while the last one leaves.
+          // after the other, in the two places by turns, the next written while the last one leaves.  Every box is a group of
+          // copies, an empty one where it leaves by plain stores or lies behind the last column: the wait for all groups but the
+          // newest says only then that the box two before, which lay in this place, has been read.
           auto leave = [&](auto wide_tag, auto first_tag, auto pack) {
             constexpr int kWide = decltype(wide_tag)::value, kFirst = decltype(first_tag)::value;
             constexpr int kBoxes = kWide == 32 ? 1 : kCols / kWide;
@@ -705,7 +707,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
               if (lane == 0) {
                 if (c0 < p.n) tma_store_3d(&map_c, at, c0, row, p.terms ? x.group : 0);
                 if (kBoxes == 2 && c0 + kWide < p.n) tma_store_3d(&map_c, at + 4096, c0 + kWide, row, p.terms ? x.group : 0);
-                bulk_commit_group();
               }
             } else {
 #pragma unroll 1
@@ -714,6 +715,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
                 if (c < p.n) store_box(p, at + b * 4096, (p.terms ? x.group * p.stride_c : 0) + row * p.ldc + c, rows, p.n - c, lane);
               }
             }
+            if (lane == 0) bulk_commit_group();
           };
           using std::integral_constant;
           if (p.out_dtype == PMLB_F32) {

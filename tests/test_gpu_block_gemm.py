@@ -220,6 +220,57 @@ def test_groups_that_share_one_b(tiles):
     check(c, *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], 128), k, K.F32)
 
 
+def again_and_again(plan, x, c, offsets=None, calls=40):
+    """Calls into a matrix that is wiped before each: every one gives the bits of the first."""
+    first, bad = c.clone(), torch.zeros((), dtype=torch.bool, device="cuda")
+    for _ in range(calls):
+        c.fill_(3.0)
+        run(plan, x, c, offsets)
+        bad |= (c != first).any()
+    plan.check()
+    assert not bad
+
+
+@pytest.mark.parametrize("tiles", [K.BLOCK_TILES_SINGLE, K.BLOCK_TILES_PAIR])
+@pytest.mark.parametrize("k", [100, 700])
+@pytest.mark.parametrize("n", [45, 66, 93, 173, 207, 301, 335, 366])
+@pytest.mark.parametrize("m", [1, 257, 20001])
+def test_f32_rows_that_end_inside_a_box(m, n, k, tiles):
+    """f32 results leave in boxes of 32 columns, in two places by turns: whole ones by TMA, one that ends inside 16 bytes by plain
+    stores, those behind the last column not at all, on rows that start on 16 bytes all the same."""
+    x = make(m, n, k, seed=n)
+    ldc = (n + 3) // 4 * 4 + 4
+    c = torch.full((m + 1, ldc), 3.0, device="cuda")
+    plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.F32, m, n, k, lda=x["ld"], ldb=x["ld"], ldc=ldc, tiles=tiles))
+    run(plan, x, c)
+    plan.check()
+    check(c[:m, :n], *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], 128), k, K.F32)
+    assert (c[:, n:] == 3).all() and (c[m] == 3).all()
+    again_and_again(plan, x, c)
+
+
+@pytest.mark.parametrize("tiles", [K.BLOCK_TILES_SINGLE, K.BLOCK_TILES_PAIR])
+@pytest.mark.parametrize("n", [264, 512, 2048])
+@pytest.mark.parametrize("whole", [128, 256])
+def test_f32_groups_whose_tails_follow_whole_tiles(whole, n, tiles):
+    """Boxes of whole tiles leave by TMA, those of a group's last rows by plain stores from the same places."""
+    counts = [whole * (g % 3) + (11 * g) % 32 for g in range(96)]
+    groups, m, k = len(counts), sum(counts), 128
+    x = make(m, n, k, each=(groups,), seed=n)
+    offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    c = torch.full((m, n), 3.0, device="cuda")
+    plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.F32, m, n, k, groups=groups, tiles=tiles))
+    run(plan, x, c, offsets)
+    plan.check()
+    at = 0
+    for g, count in enumerate(counts):
+        if count:
+            rows = slice(at, at + count)
+            check(c[rows], *expect(x["a"][rows], x["sa"][:, rows], x["b"][g], x["sb"][g], 128), k, K.F32)
+        at += count
+    again_and_again(plan, x, c, offsets)
+
+
 def test_offsets_outside_the_rows_are_taken_as_the_edge():
     m, n, k = 40, 130, 256
     x = make(m, n, k, each=(4,), seed=2)

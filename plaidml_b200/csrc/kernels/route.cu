@@ -652,7 +652,7 @@ __device__ __forceinline__ void order_pairs(const OrderParams& p, uint32_t* coun
 }
 
 __global__ void __launch_bounds__(kOrderThreads, 1) route_order_kernel(const OrderParams p) {
-  extern __shared__ uint32_t order_smem_raw[];
+  extern __shared__ __align__(16) uint32_t order_smem_raw[];
   dependent_entry();
   order_pairs(p, order_smem_raw);
 }
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kOrderThreads, 1) route_order_kernel(const Ord
 // Few tokens: one CTA chooses for them and puts the pairs in order, one launch instead of two.
 template <class T, int N>
 __global__ void __launch_bounds__(kOrderThreads, 1) route_few_kernel(const __grid_constant__ RouteParams p, const OrderParams q) {
-  extern __shared__ uint32_t order_smem_raw[];
+  extern __shared__ __align__(16) uint32_t order_smem_raw[];   // (aligned for rows of doubles: the arrays before it end 4 mod 8)
   dependent_entry();
   // (the counts come after the choice: its rows may take their place)
   const int warp = threadIdx.x >> 5;

@@ -318,6 +318,29 @@ def test_order_without_tokens():
         K.Plan("route", K.route_desc(K.F32, 4, 8, 2, K.ROUTE_SOFTMAX)).route_order(w.data_ptr(), w.data_ptr(), w.data_ptr(), w.data_ptr())
 
 
+@pytest.mark.parametrize("score", [K.ROUTE_SOFTMAX, K.ROUTE_SIGMOID])
+@pytest.mark.parametrize("experts, groups, top_groups, top_k", [(160, 4, 2, 6), (60, 4, 1, 5), (250, 5, 3, 8), (96, 32, 7, 8), (9, 3, 2, 4)])
+@pytest.mark.parametrize("tokens", [1, 33, 64, 65])
+def test_few_tokens_chosen_in_64_bits_by_groups_of_any_size(tokens, experts, groups, top_groups, top_k, score):
+    """Choice and order of few tokens (one launch up to 64), groups that are no runs of whole lanes, scores that 32 bits cannot tell apart."""
+    g = np.random.Generator(np.random.PCG64(experts))
+    z = (1 + g.standard_normal((tokens, experts)) * 1e-7).astype(np.float32)
+    z[::3] = g.standard_normal((len(z[::3]), experts))
+    bias = (g.integers(-3, 4, experts) * 2.0 ** -26).astype(np.float32)
+    rows = K.route_rows(tokens, experts, top_k, 8)
+    dev, b = torch.from_numpy(z).cuda(), torch.from_numpy(bias).cuda()
+    w, ids = torch.full((tokens, top_k), -1.0, device="cuda"), torch.full((tokens, top_k), -7, dtype=torch.int32, device="cuda")
+    offsets, source, position = (torch.full(s, -9, dtype=torch.int32, device="cuda") for s in ((experts + 1,), (rows,), (tokens, top_k)))
+    plan = K.Plan("route", K.route_desc(K.F32, tokens, experts, top_k, score, groups=groups, top_groups=top_groups, rows=rows, align=8))
+    plan.route(dev.data_ptr(), b.data_ptr(), w.data_ptr(), ids.data_ptr(), offsets.data_ptr(), source.data_ptr(), position.data_ptr())
+    torch.cuda.synchronize()
+    want_w, want_ids = routed(z, bias, top_k, score, groups, top_groups, True, 1.0)
+    assert np.array_equal(ids.cpu().numpy(), want_ids)
+    assert (np.abs(w.cpu().numpy() - want_w) <= 64 * U * want_w).all()
+    for got, want in zip((offsets, source, position), ordered(want_ids, experts, 8, rows)):
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
 @pytest.mark.parametrize("tokens", [6, 2000])
 def test_routing_in_streams_and_graphs(tokens):
     """Two graphs of one plan, replayed at the same time: each gives what the plain call gives."""

@@ -333,7 +333,7 @@ def block_gemm_desc(a_dtype: int, b_dtype: int, out_dtype: int, m: int, n: int, 
                     a_scale_row=None, a_scale_block=None, b_scale_row=None, b_scale_block=None, b_scale_group=None,
                     tiles: int = 0) -> BlockGemmDesc:
     """Defaults: dense matrices and groups; the scales of A as [blocks][m], those of B as [n / 128][blocks]
-    (b_scale_rows = 128) or [blocks][n] (b_scale_rows = 1)."""
+    (b_scale_rows = 128) or [blocks][n] (b_scale_rows = 1).  stride_b = 0 (groups of rows with one B): one set of its scales."""
     d = BlockGemmDesc()
     d.a_dtype, d.b_dtype, d.out_dtype, d.m, d.n, d.k = a_dtype, b_dtype, out_dtype, m, n, k
     d.groups, d.group_dim, d.b_scale_rows, d.tiles = groups, group_dim, b_scale_rows, tiles
@@ -345,7 +345,10 @@ def block_gemm_desc(a_dtype: int, b_dtype: int, out_dtype: int, m: int, n: int, 
     by_tile = b_scale_rows == 128
     d.b_scale_row = (_blocks(k) if by_tile else 1) if b_scale_row is None else b_scale_row
     d.b_scale_block = (1 if by_tile else n) if b_scale_block is None else b_scale_block
-    d.b_scale_group = (_blocks(n) if by_tile else n) * _blocks(k) if b_scale_group is None else b_scale_group
+    if b_scale_group is None:
+        shared = d.stride_b == 0 and group_dim == GROUP_ROWS
+        b_scale_group = 0 if shared else (_blocks(n) if by_tile else n) * _blocks(k)
+    d.b_scale_group = b_scale_group
     return d
 
 

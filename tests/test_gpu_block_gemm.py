@@ -220,6 +220,20 @@ def test_groups_that_share_one_b(tiles):
     check(c, *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], 128), k, K.F32)
 
 
+@pytest.mark.parametrize("b_rows", [1, 128])
+@pytest.mark.parametrize("tiles", TILES)
+def test_groups_that_share_one_b_and_its_scales_by_default(tiles, b_rows):
+    m, n, k, counts = 210, 136, 300, [3, 150, 0, 57]
+    x = make(m, n, k, b_rows=b_rows, seed=6)
+    offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    c = torch.empty((m, n), dtype=torch.float32, device="cuda")
+    d = K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.F32, m, n, k, lda=x["ld"], ldb=x["ld"], groups=4, stride_b=0, b_scale_rows=b_rows, tiles=tiles)
+    plan = K.Plan("block_gemm", d)
+    run(plan, x, c, offsets)
+    plan.check()
+    check(c, *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], b_rows), k, K.F32)
+
+
 def again_and_again(plan, x, c, offsets=None, calls=40):
     """Calls into a matrix that is wiped before each: every one gives the bits of the first."""
     first, bad = c.clone(), torch.zeros((), dtype=torch.bool, device="cuda")

@@ -120,6 +120,17 @@ def test_defaults_of_the_helpers_fit_one_another():
     assert K.route_rows(10, 64, 4, 128) == 40 + 40 * 127
 
 
+@pytest.mark.parametrize("b_scale_rows", [1, 128])
+def test_groups_that_share_one_b_share_its_scales(b_scale_rows):
+    def desc(**how):
+        return K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.BF16, 300, 700, 512, groups=4, b_scale_rows=b_scale_rows, **how)
+
+    whole = 700 * 4 if b_scale_rows == 1 else 6 * 4
+    assert desc(stride_b=0).b_scale_group == 0
+    assert desc().b_scale_group == whole and desc(stride_b=700 * 512 + 16).b_scale_group == whole
+    assert desc(stride_b=0, b_scale_group=5).b_scale_group == 5
+
+
 def test_null_arguments():
     lib = K.load()
     for kind in ("block_gemm", "quant", "route", "combine"):

@@ -239,14 +239,15 @@ __device__ __forceinline__ bool choose(const RouteParams& p, const float (&z)[N]
       const F worst = -warp_max(stays ? -value : kNone), rest = warp_max(group < p.groups && !stays ? value : kNone);
       close = worst - rest <= 2 * base + 4 * u * warp_max(size);
     }
+    // (the others' experts are taken, not minus infinity: that is what a bias may leave of an expert that stays)
     if (p.lanes_per_group > 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = stays || i >= held ? r[i] : kNone;
+      for (int i = 0; i < N; ++i) r[i] = stays ? r[i] : kTaken;
     } else {
       const unsigned kept = __ballot_sync(kAll, stays);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (i < held && !((kept >> ((lane * N + i) / p.group_size)) & 1u)) r[i] = kNone;
+        if (i < held && !((kept >> ((lane * N + i) / p.group_size)) & 1u)) r[i] = kTaken;
       }
     }
   }

@@ -160,6 +160,59 @@ def test_experts_that_a_bias_takes_out():
     assert np.array_equal(ids, want_ids) and (np.abs(w - want_w) <= 64 * U * want_w).all()
 
 
+def routed_among_the_groups_that_stay(z, bias, top_k, score, groups, top_groups, renormalise=True):
+    """(weights, ids) in 64 bits, each token's choice made among the experts of its groups alone."""
+    _, s = score64(z, score)
+    ids = np.empty((len(z), top_k), np.int64)
+    rank = s + np.where(np.isnan(bias), -np.inf, bias.astype(np.float64))
+    size = z.shape[1] // groups
+    for t in range(len(z)):
+        value = np.array([np.sort(rank[t, g * size: (g + 1) * size])[::-1][:2].sum() for g in range(groups)])
+        stay = np.sort(np.argsort(-value, kind="stable")[:top_groups])
+        among = np.concatenate([np.arange(g * size, (g + 1) * size) for g in stay])
+        ids[t] = among[np.argsort(-rank[t, among], kind="stable")[:top_k]]
+    w = np.take_along_axis(s, ids, 1)
+    return (w / w.sum(1, keepdims=True) if renormalise else w), ids
+
+
+@pytest.mark.parametrize("score", [K.ROUTE_SOFTMAX, K.ROUTE_SIGMOID])
+@pytest.mark.parametrize("out", [-np.inf, np.nan])
+@pytest.mark.parametrize("near", [False, True])
+@pytest.mark.parametrize("experts, groups, top_groups, top_k", [(8, 2, 1, 4), (64, 4, 1, 16), (64, 8, 2, 12), (60, 4, 2, 28), (160, 4, 1, 32),
+                                                                (256, 8, 1, 32), (32, 32, 5, 5), (1024, 16, 1, 32)])
+def test_experts_that_a_bias_takes_out_make_no_room_for_other_groups(experts, groups, top_groups, top_k, near, out, score):
+    """Fewer experts with a finite score than choices in the groups that stay: the others of these groups, not of the rest.
+    `near`: scores that 32 bits cannot tell apart, so that the choice is made in 64."""
+    g = np.random.Generator(np.random.PCG64(experts + top_k))
+    z = (g.standard_normal((50, experts)) * (1e-7 if near else 2)).astype(np.float32)
+    bias = (g.integers(-3, 4, experts) * 2.0 ** -26).astype(np.float32)
+    size = experts // groups
+    for e in range(groups):       # of each group at least one stays, and where it has them two, so that its value is finite
+        at = e * size + g.permutation(size)
+        bias[at[2 if size > 2 else size:][: (2 * size) // 3]] = out
+    w, ids = route(torch.from_numpy(z), bias, top_k, score, groups=groups, top_groups=top_groups)
+    want_w, want_ids = routed_among_the_groups_that_stay(z, bias, top_k, score, groups, top_groups)
+    assert np.array_equal(ids, want_ids)
+    assert (np.abs(w - want_w) <= 64 * U * want_w).all()
+
+
+@pytest.mark.parametrize("score", [K.ROUTE_SOFTMAX, K.ROUTE_SIGMOID])
+@pytest.mark.parametrize("tokens", [5, 100])
+def test_a_group_that_a_bias_takes_out_whole(tokens, score):
+    """All experts of the groups that stay are taken out (no group has a finite value): the first groups', in their order."""
+    experts, groups, top_groups, top_k = 64, 4, 2, 20
+    z = logits_of(tokens, experts, K.F32, 12)
+    w, ids = route(z, np.full(experts, -np.inf, np.float32), top_k, score, groups=groups, top_groups=top_groups)
+    want_w, want_ids = routed_among_the_groups_that_stay(z.numpy(), np.full(experts, -np.inf, np.float32), top_k, score, groups, top_groups)
+    assert np.array_equal(ids, want_ids) and (ids == np.arange(top_k)).all()
+    assert (np.abs(w - want_w) <= 64 * U * want_w).all()
+    bias = np.zeros(experts, np.float32)
+    bias[:16] = -np.inf            # the first group's: it never stays
+    w, ids = route(z, bias, top_k, score, groups=groups, top_groups=3)
+    _, want_ids = routed_among_the_groups_that_stay(z.numpy(), bias, top_k, score, groups, 3)
+    assert np.array_equal(ids, want_ids) and (ids >= 16).all()
+
+
 # ---------------------------------------------------------------------------------------- gradient
 
 

@@ -552,7 +552,7 @@ pmlb_status pmlb_quant_invoke(pmlb_plan* plan, void* stream, const void* x, cons
  *   experts are `groups` runs of equal length; a group's value is the sum of its two largest r (of its only one); the
  *   top_groups groups of the largest values stay
  *   ids = the top_k experts of the largest r in them, in descending order, ties to the lowest index (of the group, too)
- *   weights[j] = scale * s[ids[j]], with `renormalise` divided by the sum over the token's choices
+ *   weights[j] = scale * s[ids[j]], with `renormalise` divided by the sum over the token's choices; scale is finite in f32
  * What is chosen is what these definitions give in 64-bit arithmetic: choices that 32 bits leave open are made again in 64.
  * NaN counts as minus infinity, a sigmoid below e^-709 as zero; a token whose chosen scores are all zero has
  * zero weights.  The bias (f32, may be NULL)

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <new>
@@ -1585,7 +1586,7 @@ std::string route_problem(const pmlb_route_desc& d) {
   if (d.top_groups <= 0 || d.top_groups > d.groups) return "route: top_groups must be 1..groups";
   if (d.top_k > d.experts / d.groups * d.top_groups) return "route: more choices than experts to choose from";
   if (d.ld < d.experts) return "route: a row stride smaller than a row";
-  if (!(d.scale - d.scale == 0.0)) return "route: scale is not finite";
+  if (!std::isfinite(static_cast<float>(d.scale))) return "route: scale is not finite in f32";
   const long long pairs = static_cast<long long>(d.tokens) * d.top_k;
   if (pairs > (1 << 24)) return "route: more than 2^24 pairs";
   if (d.rows < 0 || (d.rows > 0 && (d.align < 1 || d.align > 1024))) return "route: rows must not be negative, align 1..1024";

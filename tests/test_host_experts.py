@@ -85,6 +85,16 @@ def test_routings_that_are_refused(fields, word):
     assert word in problem("route", route(**fields))
 
 
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.5e38, float("nan")])
+def test_scales_of_weights_that_f32_cannot_hold_are_refused(scale):
+    assert "finite" in problem("route", route(scale=scale))
+
+
+def test_the_largest_scale_of_weights_is_taken():
+    assert problem("route", route(scale=3.4028234e38)) is None
+    assert problem("route", route(scale=-3.4028234e38)) is None and problem("route", route(scale=0.0)) is None
+
+
 def test_routings_that_are_taken():
     assert problem("route", route()) is None
     assert problem("route", route(rows=K.route_rows(100, 64, 8, 16) // 16 * 16)) is None

@@ -322,6 +322,14 @@ __device__ __noinline__ int choose_again(const RouteParams& p, long long t, int 
   return id;
 }
 
+// e^(z - m), m >= z.  The difference's rounding is as much as |z - m| / 2 units of the last place of the exponential, so what it leaves
+// out (Knuth's sum of two numbers: exact) goes into the result.
+__device__ __forceinline__ float exp_between(float z, float m) {
+  const float d = z - m, e = expf(d);
+  const float back = d - z, rest = (z - (d - back)) - (m + back);
+  return d > -128.f ? fmaf(e, rest, e) : e;   // (0 below; and the rest of an infinity is none)
+}
+
 // The chosen experts' weights before `scale`, lane j the j-th one's: scores over the row, or (renormalise) shares of the choice.
 // `rest`: 1 - score for sigmoid.
 template <class T, int N>
@@ -335,7 +343,7 @@ __device__ __forceinline__ float weight_of(const RouteParams& p, long long t, in
     if (!p.renormalise) return mine ? 1.f / (1.f + expf(-zc)) : 0.f;
     // Shares of scores that may all underflow in 32 bits: relative to e^m, m the largest logit or 0.
     const float m = fminf(warp_max(zc), 0.f);
-    if (zc >= kNoScore) w = zc < 0.f ? expf(zc - m) / (1.f + expf(zc)) : 1.f / (1.f + expf(-zc));
+    if (zc >= kNoScore) w = zc < 0.f ? exp_between(zc, m) / (1.f + expf(zc)) : 1.f / (1.f + expf(-zc));
   } else {
     float m = zc;
     if (!p.renormalise) {
@@ -343,12 +351,12 @@ __device__ __forceinline__ float weight_of(const RouteParams& p, long long t, in
       for (int i = 0; i < N; ++i) m = fmaxf(m, z[i]);
     }
     m = fmaxf(warp_max(m), -FLT_MAX);
-    w = expf(zc - m);
+    w = exp_between(zc, m);
     if (!p.renormalise) {
-      // (the sum's terms that matter have small arguments, which the fast exponential takes as exactly)
+      // (the plain difference will do here: its rounding is worth u |z - m| of a term that is e^(z - m) of the sum or less)
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum += exp2_fast((z[i] - m) * kLog2e);
+      for (int i = 0; i < N; ++i) sum += expf(z[i] - m);
       sum = warp_sum(sum);
       return sum > 0.f ? w / sum : 0.f;
     }

@@ -160,6 +160,21 @@ def test_experts_that_a_bias_takes_out():
     assert np.array_equal(ids, want_ids) and (np.abs(w - want_w) <= 64 * U * want_w).all()
 
 
+@pytest.mark.parametrize("score, renormalise", [(K.ROUTE_SOFTMAX, True), (K.ROUTE_SOFTMAX, False), (K.ROUTE_SIGMOID, True)])
+@pytest.mark.parametrize("experts", [2, 3])
+def test_weights_of_experts_far_below_the_first(experts, score, renormalise):
+    """Small weights are as accurate as large ones.  An exponential is within one last place of the rounded one (3 u) and takes
+    what its argument's rounding left out (2 u more); of sigmoids it is divided by a sum (3 u and u), and u for that: 10 u; the sum
+    of two or three of them 10 u of a weighted mean, two u for additions, u for the quotient: 23 u."""
+    g = np.random.Generator(np.random.PCG64(experts))
+    first = -g.random((20000, 1)) * 3 - 0.1
+    z = np.concatenate([first, first - g.random((20000, experts - 1)) * 80], 1).astype(np.float32)
+    w, ids = route(torch.from_numpy(z), None, experts, score, renormalise=renormalise)
+    want, want_ids = routed(z, None, experts, score, 1, 1, renormalise, 1.0)
+    assert np.array_equal(ids, want_ids)
+    assert (np.abs(w - want) <= 23 * U * want).all(), (np.abs(w - want) / want).max() / U
+
+
 def routed_among_the_groups_that_stay(z, bias, top_k, score, groups, top_groups, renormalise=True):
     """(weights, ids) in 64 bits, each token's choice made among the experts of its groups alone."""
     _, s = score64(z, score)

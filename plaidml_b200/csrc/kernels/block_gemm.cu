@@ -938,9 +938,10 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   p.bs_row = d.b_scale_row, p.bs_block = d.b_scale_block, p.bs_group = d.b_scale_group;
   p.b_shift = d.b_scale_rows == 128 ? 7 : 0;
   p.b_step = by_rows && d.stride_b == 0 ? 0 : 1;
-  p.out = c, p.ldc = d.ldc, p.stride_c = d.stride_c, p.out_dtype = d.out_dtype;
+  const bool many_c = by_terms && d.groups > 1;   // (a single group has no neighbour)
+  p.out = c, p.ldc = d.ldc, p.stride_c = many_c ? d.stride_c : 0, p.out_dtype = d.out_dtype;
   const long long ob = d.out_dtype == PMLB_F32 ? 4 : 2;
-  const long long bits = static_cast<long long>(reinterpret_cast<uintptr_t>(c)) | (d.ldc * ob) | (by_terms ? d.stride_c * ob : 0);
+  const long long bits = static_cast<long long>(reinterpret_cast<uintptr_t>(c)) | (d.ldc * ob) | (p.stride_c * ob);
   p.out_align = bits % 32 == 0 ? 32 : (bits % 16 == 0 ? 16 : 1);
   p.status = status;
 
@@ -971,7 +972,7 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   const bool many_b = by_rows && d.stride_b != 0;
   if (!tc_encode_bytes(&mb, b, d.k, d.n, many_b ? d.groups : 1, d.ldb, many_b ? d.stride_b : 16, box_b, err)) return PMLB_ERR_INVALID;
   if (!swap && p.out_align >= 16 &&
-      !tc_encode_boxes(&mc, d.out_dtype, c, d.n, d.m, by_terms ? d.groups : 1, d.ldc, by_terms ? d.stride_c : 8, err)) {
+      !tc_encode_boxes(&mc, d.out_dtype, c, d.n, d.m, many_c ? d.groups : 1, d.ldc, many_c ? d.stride_c : 8, err)) {
     return PMLB_ERR_INVALID;
   }
   cudaError_t e = cudaSuccess;

@@ -220,6 +220,21 @@ def test_groups_that_share_one_b(tiles):
     check(c, *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], 128), k, K.F32)
 
 
+@pytest.mark.parametrize("stride_c", [0, 4, -8, 1 << 39])
+@pytest.mark.parametrize("tiles", [0] + TILES)
+def test_one_group_of_terms_whatever_its_stride(tiles, stride_c):
+    """A single group has no neighbour: the distance to it counts for nothing."""
+    m, n, k, lo, hi = 200, 264, 640, 128, 512
+    x = make(m, n, k, b_rows=1, seed=8)
+    offsets = torch.tensor([lo, hi], dtype=torch.int32, device="cuda")
+    c = torch.full((m, n), 3.0, device="cuda")
+    plan = K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.F32, m, n, k, groups=1, group_dim=K.GROUP_TERMS, b_scale_rows=1,
+                                                  stride_c=stride_c, tiles=tiles))
+    run(plan, x, c, offsets)
+    plan.check()
+    check(c, *expect(x["a"][:, lo:hi], x["sa"][1:4], x["b"][:, lo:hi], x["sb"][1:4], 1), hi - lo, K.F32)
+
+
 @pytest.mark.parametrize("b_rows", [1, 128])
 @pytest.mark.parametrize("tiles", TILES)
 def test_groups_that_share_one_b_and_its_scales_by_default(tiles, b_rows):

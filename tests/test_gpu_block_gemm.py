@@ -220,6 +220,56 @@ def test_groups_that_share_one_b(tiles):
     check(c, *expect(x["a"][:, :k], x["sa"], x["b"][:, :k], x["sb"], 128), k, K.F32)
 
 
+@pytest.mark.parametrize("out", [K.F16, K.BF16, K.F32])
+@pytest.mark.parametrize("b_rows", [1, 128])
+@pytest.mark.parametrize("a, b", [(K.F8E5M2, K.F8E4M3), (K.F8E4M3, K.F8E5M2)])
+@pytest.mark.parametrize("tiles", [0] + TILES)
+def test_groups_of_rows_types_and_scales_of_each_row(tiles, a, b, b_rows, out):
+    """Each group's scales of B: [blocks][n] or [n / 128][blocks], a set behind the other and, here, a gap behind each."""
+    counts = [3, 0, 130, 257, 0, 1, 40]
+    groups, m, n, k = len(counts), sum(counts), 200, 600
+    x = make(m, n, k, a, b, b_rows, each=(groups,), seed=21)
+    sets = x["sb"]
+    wide = torch.full((groups, sets[0].numel() + 3), float("nan"), device="cuda")
+    wide[:, :-3] = sets.reshape(groups, -1)
+    x["sb"] = wide
+    offsets = torch.tensor([0] + counts).cumsum(0).int().cuda()
+    c = torch.full((m, n), 3.0, dtype=TORCH_OF[out], device="cuda")
+    plan = K.Plan("block_gemm", K.block_gemm_desc(a, b, out, m, n, k, lda=x["ld"], ldb=x["ld"], groups=groups, b_scale_rows=b_rows,
+                                                  b_scale_group=wide.shape[1], tiles=tiles))
+    run(plan, x, c, offsets)
+    plan.check()
+    at = 0
+    for g, count in enumerate(counts):
+        if count:
+            rows = slice(at, at + count)
+            check(c[rows], *expect(x["a"][rows, :k], x["sa"][:, rows], x["b"][g, :, :k], sets[g], b_rows), k, out)
+        at += count
+
+
+@pytest.mark.parametrize("out", [K.F16, K.BF16])
+@pytest.mark.parametrize("b_rows", [1, 128])
+@pytest.mark.parametrize("a, b", [(K.F8E5M2, K.F8E4M3), (K.F8E5M2, K.F8E5M2)])
+@pytest.mark.parametrize("tiles", [0] + TILES)
+def test_groups_of_terms_types_and_scales_of_128_rows(tiles, a, b, b_rows, out):
+    counts, m, n = [2, 0, 5, 1], 150, 330
+    groups, k = len(counts), 128 * sum(counts)
+    x = make(m, n, k, a, b, b_rows, seed=22)
+    offsets = (torch.tensor([0] + counts).cumsum(0) * 128).int().cuda()
+    c = torch.full((groups, m, n), 3.0, dtype=TORCH_OF[out], device="cuda")
+    plan = K.Plan("block_gemm", K.block_gemm_desc(a, b, out, m, n, k, groups=groups, group_dim=K.GROUP_TERMS, b_scale_rows=b_rows, tiles=tiles))
+    run(plan, x, c, offsets)
+    plan.check()
+    for g in range(groups):
+        lo, hi = int(offsets[g]), int(offsets[g + 1])
+        if hi > lo:
+            blocks_of = slice(lo // 128, hi // 128)
+            sb = x["sb"][blocks_of] if b_rows == 1 else x["sb"][:, blocks_of]
+            check(c[g], *expect(x["a"][:, lo:hi], x["sa"][blocks_of], x["b"][:, lo:hi], sb, b_rows), hi - lo, out)
+        else:
+            assert (c[g] == 0).all()
+
+
 @pytest.mark.parametrize("stride_c", [0, 4, -8, 1 << 39])
 @pytest.mark.parametrize("tiles", [0] + TILES)
 def test_one_group_of_terms_whatever_its_stride(tiles, stride_c):

@@ -6,6 +6,10 @@ less than u, relative to the largest), sums of at most 1024 of them in chains of
 64 u of the weight.  The gradient adds a product sum over at most 32 choices, another 70 u of the sum of absolute
 values.  Sums over rows: one u per term of the sum of absolute values.  Results in 16 bits: half a step more."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -448,6 +452,59 @@ def test_routing_in_streams_and_graphs(tokens):
     torch.cuda.synchronize()
     for x, y in zip(sets, want):
         assert all(torch.equal(x[k], y[k]) for k in x)
+
+
+FIRST_CALL = """
+import torch
+from plaidml_b200 import kernels as K
+z, w, ids = torch.randn((TOKENS, 64), device="cuda"), torch.zeros((TOKENS, 4), device="cuda"), torch.zeros((TOKENS, 4), dtype=torch.int32, device="cuda")
+offsets, source, position = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (65, 4 * TOKENS, 4 * TOKENS))
+x, y = (torch.randn((4 * TOKENS, 256), device="cuda").bfloat16() for _ in range(2))
+q = torch.zeros((4 * TOKENS, 256), dtype=torch.uint8, device="cuda")
+s, sb = torch.ones((2, 4 * TOKENS), device="cuda"), torch.ones((64, 2, 2), device="cuda")
+b = torch.zeros((64, 256, 256), dtype=torch.uint8, device="cuda")
+c, out = torch.zeros((4 * TOKENS, 256), dtype=torch.bfloat16, device="cuda"), torch.zeros((TOKENS, 256), dtype=torch.bfloat16, device="cuda")
+dz, dw, dy = torch.zeros_like(z), torch.zeros_like(w), torch.zeros_like(x)
+
+def all_of_it(stream):
+    plans = [K.Plan("route", K.route_desc(K.F32, TOKENS, 64, 4, K.ROUTE_SOFTMAX, rows=4 * TOKENS)),
+             K.Plan("quant", K.quant_desc(K.BF16, K.F8E4M3, 4 * TOKENS, 256, K.QUANT_ROWS)),
+             K.Plan("block_gemm", K.block_gemm_desc(K.F8E4M3, K.F8E4M3, K.BF16, 4 * TOKENS, 256, 256, groups=64)),
+             K.Plan("combine", K.combine_desc(K.BF16, TOKENS, 4, 256, 4 * TOKENS))]
+    at = [t.data_ptr() for t in (z, w, ids, offsets, source, position)]
+    plans[0].route(at[0], None, *at[1:], stream=stream)
+    plans[1].quant(x.data_ptr(), q.data_ptr(), s.data_ptr(), stream=stream)
+    plans[2].block_gemm(q.data_ptr(), s.data_ptr(), b.data_ptr(), sb.data_ptr(), c.data_ptr(), offsets=at[3], stream=stream)
+    plans[3].combine(y.data_ptr(), at[1], at[5], out.data_ptr(), stream=stream)
+    plans[3].combine_grad(out.data_ptr(), y.data_ptr(), at[1], at[5], at[4], dy.data_ptr(), dw.data_ptr(), stream=stream)
+    plans[0].route_grad(at[0], at[2], dw.data_ptr(), dz.data_ptr(), stream=stream)
+    return plans
+
+results = (w, ids, offsets, source, position, q, s, c, out, dy, dw, dz)
+b.copy_(torch.randint(0, 100, b.shape, dtype=torch.uint8, device="cuda"))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    plans = all_of_it(torch.cuda.current_stream().cuda_stream)
+del plans
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in results]
+for t in results:
+    t.zero_()
+plans = all_of_it(0)
+torch.cuda.synchronize()
+assert all(torch.equal(a, t) for a, t in zip(got, results)) and float(out.abs().max()) > 0
+print("alike")
+"""
+
+
+@pytest.mark.parametrize("tokens", [8, 1000])
+def test_plans_made_and_called_for_the_first_time_under_capture(tokens):
+    """In a process of its own: nothing of the library has run on the device before the capture, and the plans are gone before the replay."""
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL.replace("TOKENS", str(tokens))], capture_output=True, text=True, timeout=300,
+                          cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0 and "alike" in done.stdout, done.stderr[-2000:]
 
 
 # ---------------------------------------------------------------------------------------- combination

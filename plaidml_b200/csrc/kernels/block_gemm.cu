@@ -82,7 +82,7 @@ struct BlockGemmParams {
   int b_step;              // 1, or 0 where all groups share one B
   void* out;
   long long ldc, stride_c;
-  int out_dtype, out_align;   // bytes that every row and the matrix start on: 32, 16, or less
+  int out_dtype, out_wide;   // every row and the matrix start on 16 bytes
   int split;               // CTAs of a cluster that share the tile's blocks
   uint32_t idesc;
   int* status;
@@ -187,7 +187,7 @@ __device__ __forceinline__ void store_one(const BlockGemmParams& p, long long at
 
 // Four consecutive columns of a row from element `at` on, `n` of which exist.
 __device__ __forceinline__ void store_four(const BlockGemmParams& p, long long at, const float4& v, int n) {
-  if (n >= 4 && p.out_align >= 16) {
+  if (n >= 4 && p.out_wide) {
     if (p.out_dtype == PMLB_F32) {
       *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
     } else {
@@ -230,7 +230,7 @@ __device__ __forceinline__ void store_box(const BlockGemmParams& p, uint32_t at,
   const int bytes = p.out_dtype == PMLB_F32 ? 4 : 2;
   char* dst = static_cast<char*>(p.out) + base * bytes;
   const long long step = p.ldc * bytes;
-  if (n * bytes >= 128 && p.out_align >= 16) {
+  if (n * bytes >= 128 && p.out_wide) {
     const int piece = lane & 7;
 #pragma unroll 4
     for (int r = lane >> 3; r < 32; r += 4) {
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
   } else if (threadIdx.x == 96) {
     tma_prefetch_desc(&map_p);
     tma_prefetch_desc(&map_q);
-    if (!SWAP && p.out_align >= 16) tma_prefetch_desc(&map_c);
+    if (!SWAP && p.out_wide) tma_prefetch_desc(&map_c);
   } else if (warp == 1) {
     if constexpr (PAIR) {
       tmem_alloc_pair(smem_u32(tmem_slot), Cfg::kTmemCols);
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1)
         if (rows > 0) {
           const uint32_t places = out_stage + static_cast<uint32_t>(w) * 8192u;
           // (a box that holds rows of the next group is stored row by row)
-          const bool by_tma = p.out_align >= 16 && (rows == 32 || x.row_end == p.m);
+          const bool by_tma = p.out_wide && (rows == 32 || x.row_end == p.m);
           // 16 bits: the warp's boxes of 64 columns together, one fence and one group of copies.  f32: boxes of 32 columns one
           // after the other, in the two places by turns, the next written while the last one leaves.  Every box is a group of
           // copies, an empty one where it leaves by plain stores or lies behind the last column: the wait for all groups but the
@@ -942,7 +942,7 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   p.out = c, p.ldc = d.ldc, p.stride_c = many_c ? d.stride_c : 0, p.out_dtype = d.out_dtype;
   const long long ob = d.out_dtype == PMLB_F32 ? 4 : 2;
   const long long bits = static_cast<long long>(reinterpret_cast<uintptr_t>(c)) | (d.ldc * ob) | (p.stride_c * ob);
-  p.out_align = bits % 32 == 0 ? 32 : (bits % 16 == 0 ? 16 : 1);
+  p.out_wide = bits % 16 == 0;
   p.status = status;
 
   const Choice choice = choose(d, dev, sms);
@@ -971,19 +971,20 @@ int block_gemm_launch(const pmlb_block_gemm_desc& d, const void* a, const float*
   if (!tc_encode_bytes(&ma, a, d.k, d.m, 1, d.lda, 16, box_a, err)) return PMLB_ERR_INVALID;
   const bool many_b = by_rows && d.stride_b != 0;
   if (!tc_encode_bytes(&mb, b, d.k, d.n, many_b ? d.groups : 1, d.ldb, many_b ? d.stride_b : 16, box_b, err)) return PMLB_ERR_INVALID;
-  if (!swap && p.out_align >= 16 &&
+  if (!swap && p.out_wide &&
       !tc_encode_boxes(&mc, d.out_dtype, c, d.n, d.m, many_c ? d.groups : 1, d.ldc, many_c ? d.stride_c : 8, err)) {
     return PMLB_ERR_INVALID;
   }
   cudaError_t e = cudaSuccess;
-  const bool both = d.b_scale_rows == 1;   // rows and columns of a tile have scales of their own
+  // Rows and columns of an accumulator have scales of their own; where its rows are rows of B, the columns are tokens, which always do.
+  const bool both = d.b_scale_rows == 1;
   if (swap) {
     if (bn == 16) {
-      e = both ? launch<BlockCfg<16, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream) : launch<BlockCfg<16, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
+      e = launch<BlockCfg<16, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
     } else if (bn == 32) {
-      e = both ? launch<BlockCfg<32, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream) : launch<BlockCfg<32, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
+      e = launch<BlockCfg<32, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
     } else {
-      e = both ? launch<BlockCfg<64, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream) : launch<BlockCfg<64, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
+      e = launch<BlockCfg<64, true, kOfBoth>>(mb, ma, mc, p, grid, dev, stream);
     }
   } else if (pair) {
     e = both ? launch<BlockCfg<256, false, kOfBoth, 2>>(ma, mb, mc, p, grid, dev, stream) : launch<BlockCfg<256, false, kOfRows, 2>>(ma, mb, mc, p, grid, dev, stream);

@@ -237,7 +237,8 @@ __device__ __forceinline__ bool choose(const RouteParams& p, const float (&z)[N]
       F size = (first < 0 ? -first : first) + (p.group_size > 1 ? (second < 0 ? -second : second) : F(0));
       if (!(size < static_cast<F>(INFINITY))) size = 0;
       const F worst = -warp_max(stays ? -value : kNone), rest = warp_max(group < p.groups && !stays ? value : kNone);
-      close = worst - rest <= 2 * base + 4 * u * warp_max(size);
+      // (two infinities: sums of two large biases that 64 bits hold)
+      close = !(worst - rest > 2 * base + 4 * u * warp_max(size));
     }
     // (the others' experts are taken, not minus infinity: that is what a bias may leave of an expert that stays)
     if (p.lanes_per_group > 0) {

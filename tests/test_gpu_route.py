@@ -232,6 +232,26 @@ def test_a_group_that_a_bias_takes_out_whole(tokens, score):
     assert np.array_equal(ids, want_ids) and (ids >= 16).all()
 
 
+@pytest.mark.parametrize("score", [K.ROUTE_SOFTMAX, K.ROUTE_SIGMOID])
+@pytest.mark.parametrize("experts, groups", [(16, 4), (60, 4), (256, 8), (15, 5)])
+def test_groups_whose_values_32_bits_cannot_hold(experts, groups, score):
+    """Biases of the largest numbers, as masks have them: the sum of two is infinite in 32 bits, but not in 64."""
+    low, high, size = np.finfo(np.float32).min, np.finfo(np.float32).max, experts // groups
+    z = logits_of(40, experts, K.F32, 13)
+    rising = (high * (0.55 + 0.4 * np.arange(experts) / experts)).astype(np.float32)     # all sums of two are infinite in 32 bits
+    for first, others in ((-np.inf, low), (high / 2, high), (high * 0.75, high), (None, None)):
+        bias = np.zeros(experts, np.float32)
+        bias[:size], bias[size: (groups - 1) * size] = first or 0, others or 0
+        if first is None:
+            bias = rising
+        for top_groups in (1, 2, 3):
+            top_k = min(32, top_groups * size - 1)
+            w, ids = route(z, bias, top_k, score, groups=groups, top_groups=top_groups)
+            want_w, want_ids = routed_among_the_groups_that_stay(z.numpy(), bias, top_k, score, groups, top_groups)
+            assert np.array_equal(ids, want_ids)
+            assert (np.abs(w - want_w) <= 64 * U * want_w).all()
+
+
 # ---------------------------------------------------------------------------------------- gradient
 
 

@@ -471,7 +471,8 @@ pmlb_status pmlb_special_invoke(pmlb_plan* plan, void* stream, const void* in0, 
  * [128 b, 128 b + 128), the last one shorter where 128 does not divide k.  A has a scale for each row and block, B for
  * each 128 rows and block (b_scale_rows = 128, j' = j / 128: weights) or for each row and block (b_scale_rows = 1, j' = j:
  * the second operand of a weight gradient).  The 128 products of a block are added on the tensor cores, the blocks, times
- * their scales, in f32 in the order of b; one rounding to out_dtype (F32, BF16 or F16).  The K range of products of few
+ * their scales, in f32 in the order of b; one rounding to out_dtype (F32, BF16 or F16).  (b_scale_rows = 128 on tiles of many
+ * rows: the product of the two scales comes first and should be a normal f32 number.)  The K range of products of few
  * rows is shared by up to eight CTAs, which adds 2..8 runs of blocks in a fixed order: results are the same on every call.
  *
  * groups = 0: one product.  groups = 1..1024 with `offsets`, int32[groups + 1] in device memory, ascending from 0:
@@ -482,7 +483,9 @@ pmlb_status pmlb_special_invoke(pmlb_plan* plan, void* stream, const void* in0, 
  *                     the experts' weight gradients, both operands transposed by PMLB_QUANT_COLUMNS.  Offsets are
  *                     multiples of 128 (see `align` of pmlb_route_desc); a group without terms gives zeros.
  * Offsets outside [0, m] (of terms: [0, k]) are taken as the nearest edge; a group that would end before it begins is empty
- * and, of rows, the next one begins where the last one ended.
+ * and, of rows, the next one begins where the last one ended.  The tiles are chosen from m and the number of groups, before the
+ * offsets are known, and all rows between offsets are computed, those that only fill a segment up, too: a batch of few tokens
+ * is routed with align = 1.
  * lda, ldb and stride_b are multiples of 16 and the operands start on 16 bytes. */
 #define PMLB_GROUP_ROWS 0
 #define PMLB_GROUP_TERMS 1
@@ -554,11 +557,12 @@ pmlb_status pmlb_quant_invoke(pmlb_plan* plan, void* stream, const void* x, cons
  *   ids = the top_k experts of the largest r in them, in descending order, ties to the lowest index (of the group, too)
  *   weights[j] = scale * s[ids[j]], with `renormalise` divided by the sum over the token's choices; scale is finite in f32
  * What is chosen is what these definitions give in 64-bit arithmetic: choices that 32 bits leave open are made again in 64.
- * The weights of a choice are computed in 32 bits: each normal one is off by less than 64 * 2^-24 of itself (a sum of up to
- * 1024 exponentials in that order of additions; 8 * 2^-24 was the most in 10^5 rows of each of 2 to 1024 experts).
- * NaN counts as minus infinity, a sigmoid below e^-709 as zero; a token whose chosen scores are all zero has
- * zero weights.  The bias (f32, may be NULL)
- * takes part in the choice alone.
+ * The weights of a choice are computed in 32 bits: each normal one is off by less than 64 * 2^-24 of itself, nearly all of it
+ * what the additions of a sum of 1024 exponentials can cost at worst (the most that 20000 rows and more of 2 to 1024 experts
+ * showed is 8 * 2^-24).  A logit that is NaN counts as minus infinity, plus infinity as the largest f32 number, a sigmoid below
+ * e^-709 as zero; a token whose chosen scores are all zero has zero weights.  The bias (f32, may be NULL) takes part in the
+ * choice alone; NaN counts as minus infinity there, too.  Experts of the groups that stay come before all others, whatever
+ * their r.
  *
  * The experts' order of the (token, choice) pairs, pair t * top_k + j going to expert ids[t, j] (`rows` > 0, else
  * the three are not computed and may be NULL):

@@ -877,11 +877,11 @@ struct Choice {
 
 // Which tiles, and how many CTAs share the blocks of one.  Few rows: weights on the accumulator's rows and as few columns as hold
 // the rows -- up to 64, or twice the average of groups, so that most groups are one tile (16 rows to each of 8 groups, 2048 x
-// 1024: 5.7 us with 32 columns, 7.9 with 16; 48 rows to each of 16: single tiles 12.4 us, few rows 17.9).  Else the smaller
-// estimate, in cycles, of pairs of CTAs on 256 x 256 and of single ones on 128 x 128.  Measured per block: pairs 700 (1150 where
-// rows and columns have scales of their own), single CTAs 540 (640), which is what an SM takes in of operands; around the blocks
-// of a tile 3300 and 1500; 6500 for clusters that add parts up.  (4096 wide and deep, pairs / single / with K split: 100 rows 17.8
-// / 13.5 / 10.1 us, 256 18.0 / 13.9 / 13.0, 1024 20.5 / 26.0.)
+// 1024: 5.7 us with 32 columns, 7.9 with 16; 48 rows to each of 16 groups, 1024 x 2048: single tiles 10.6 us, few rows 15.3).
+// Else the smaller estimate, in cycles, of pairs of CTAs on 256 x 256 and of single ones on 128 x 128.  Measured per block: pairs
+// 700 (1150 where rows and columns have scales of their own), single CTAs 540 (640), which is what an SM takes in of operands;
+// around the blocks of a tile 3300 and 1500; 6500 for clusters that add parts up.  (4096 wide and deep, pairs / single / with K
+// split: 100 rows 17.8 / 13.5 / 10.1 us, 256 18.0 / 13.9 / 13.0, 1024 20.5 / 26.0.)
 Choice choose(const pmlb_block_gemm_desc& d, int dev, int sms) {
   const bool by_rows = d.groups > 0 && d.group_dim == PMLB_GROUP_ROWS, by_terms = d.groups > 0 && !by_rows;
   const int num_kb = (d.k + kBlock - 1) / kBlock, kb = by_terms ? (num_kb + d.groups - 1) / d.groups : num_kb;

@@ -456,7 +456,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_kernel(const __gr
 // ---------------------------------------------------------------- order
 
 constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kMaxExperts = 1024;
-constexpr int kKeep = 8;   // steps of 32 pairs whose ranks a warp keeps in registers; longer runs keep theirs in `position`
+// Steps of 32 pairs whose ranks a warp keeps in registers; longer runs keep theirs in `position` and place their rows one by one.  (256
+// experts, 16 CTAs: 65536 pairs 8.4 us, 131072, which is eight steps, 11.0, 131080 12.7, 262144 20.8, 524288 37.5.)
+constexpr int kKeep = 8;
 
 struct OrderParams {
   const int32_t* ids;

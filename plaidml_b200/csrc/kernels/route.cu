@@ -700,7 +700,8 @@ cudaError_t prepare(Kernel kernel, int smem, std::atomic<uint64_t>* done, int de
 OrderParams order_of(const pmlb_route_desc& d, const int32_t* ids, int32_t* offsets, int32_t* source, int32_t* position) {
   OrderParams p{};
   p.ids = ids, p.offsets = offsets, p.source = source, p.position = position;
-  p.pairs = d.tokens * d.top_k, p.experts = d.experts, p.rows = d.rows, p.align = d.align;
+  p.pairs = d.tokens * d.top_k, p.experts = d.experts, p.rows = d.rows;
+  p.align = std::max(d.align, 1);   // (not looked at where there are no rows)
   p.ctas = 1;
   return p;
 }

@@ -433,6 +433,16 @@ def test_few_tokens_chosen_in_64_bits_by_groups_of_any_size(tokens, experts, gro
         assert np.array_equal(got.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("align", [0, -5, 1 << 30])
+def test_order_without_tokens_and_rows(align):
+    """Nothing to put in order: the offsets alone, whatever the alignment of rows that there are not."""
+    offsets = torch.full((10,), -9, dtype=torch.int32, device="cuda")
+    plan = K.Plan("route", K.route_desc(K.F32, 0, 8, 2, K.ROUTE_SOFTMAX, rows=0, align=align))
+    plan.route_order(None, offsets.data_ptr(), None, None)
+    torch.cuda.synchronize()
+    assert offsets.tolist() == [0] * 9 + [-9]
+
+
 @pytest.mark.parametrize("tokens", [6, 2000])
 def test_routing_in_streams_and_graphs(tokens):
     """Two graphs of one plan, replayed at the same time: each gives what the plain call gives."""
